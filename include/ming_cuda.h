@@ -228,6 +228,107 @@ int ming_cuda_loop_destroy(ming_loop* lp);
  * envelope and the "same" trim of 1323 samples per side. */
 int ming_cuda_vae_decode(ming_ctx* ctx, const uint16_t* latents, int T, float* wave, int ptr_kind);
 
+/* ---- operators on caller-owned paged K/V caches ----
+ *
+ * Attention with a sliding window and sinks, the weights it gives to cached
+ * positions, and eviction by those weights: what a cache of bounded size
+ * needs. A context configured with attn_window, attn_sinks or kv_track runs
+ * the same kernels in its LM steps, and ming_cuda_seq_evict on its own
+ * sequences; these entry points take the caller's device memory. They need
+ * no finalized model.
+ *
+ * Every pointer is device memory of the context's GPU. Work goes to `stream`
+ * (a cudaStream_t of that GPU; NULL = the context's stream; cudaStreamLegacy
+ * names the legacy default stream), is asynchronous, allocates nothing and
+ * can be captured into a graph. No call keeps a workspace, so calls on
+ * different streams do not disturb each other. Bad arguments are
+ * MING_ERR_INVALID; what only the device sees (a block table entry outside
+ * the pool, a length above max_len) never leaves the buffers given: the
+ * affected sequences' results are unspecified and the next ming_cuda_sync
+ * after the work returns MING_ERR_CUDA.
+ *
+ * Element (page, layer, kv head, slot, dim) of K sits at k + page *
+ * page_stride + layer * layer_stride + head * head_stride + slot *
+ * slot_stride + dim; V alike. Pages hold 16 positions, heads have 64 dims
+ * (contiguous), values are bf16. Strides count elements and are multiples
+ * of 8; k and v are 16-byte aligned. */
+typedef struct ming_kv_cache {
+    uint16_t* k;
+    uint16_t* v;
+    int64_t page_stride, layer_stride, head_stride, slot_stride;
+    int pages, layers, kv_heads;
+    int seqs;               /* sequences in the batch */
+    const int* block_table; /* [seqs][bt_ld]: positions 16 i .. 16 i + 15 of a sequence are in page [seq][i] */
+    int bt_ld;
+    int max_len;            /* no sequence holds more (at most 16 * bt_ld) */
+    const int* lens;        /* [seqs] positions held, 0 allowed */
+} ming_kv_cache;
+
+/* A row at position p of its sequence sees j <= p with j < sinks or
+ * j > p - window; window 0: every j <= p. Logits are scale * q.k (scale 0:
+ * 1/8), summed in f32; softmax in f32; out is rounded to bf16. heads is a
+ * multiple of kv_heads with at most 8 query heads per kv head. Row r, head h
+ * of q is at q + r * q_row_stride + h * q_head_stride (16-byte aligned,
+ * strides multiples of 8). A row that sees nothing gets zeros and a
+ * log-sum-exp of -infinity. */
+typedef struct ming_attn {
+    int layer, heads, window, sinks;
+    float scale;
+    const uint16_t* q;
+    int64_t q_row_stride, q_head_stride;
+    uint16_t* out;
+    int64_t out_row_stride, out_head_stride;
+    const int* q_start;     /* [seqs + 1]: sequence b's rows are [q_start[b], q_start[b + 1]) of q (prefill, weights) */
+    int rows, max_rows;     /* rows of q in all, and of the sequence with the most */
+    float* lse;             /* [rows][heads]: log sum exp of each row's logits */
+    float* acc;             /* running totals: (seq, layer, kv head, j) at acc + seq * acc_seq_stride + ... + j */
+    int64_t acc_seq_stride, acc_layer_stride, acc_head_stride;
+    void* stream;
+} ming_attn;
+
+/* Attention of a prompt's rows. The rows' own keys and values are in the
+ * cache already: the n rows of a sequence are its last n positions. Writes
+ * out and, unless NULL, lse; rows of q past the last sequence's stay as they
+ * are. acc is NULL. */
+int ming_cuda_attn_prefill(ming_ctx* ctx, const ming_kv_cache* cache, const ming_attn* attn);
+
+/* The attention weights of the same rows, added up over the rows and the
+ * query heads of a group: acc[j] = (j one of the rows' own positions ? 0 :
+ * acc[j]) + sum exp(s_ij - lse_i). Takes the lse that ming_cuda_attn_prefill
+ * gave with the same q, window, sinks and scale; out is not used. Entries at
+ * and past the sequence's length stay as they are. */
+int ming_cuda_attn_weights(ming_ctx* ctx, const ming_kv_cache* cache, const ming_attn* attn);
+
+/* Attention of one new token per sequence: row b of q is the last position
+ * of sequence b (its key and value are in the cache already). A sequence of
+ * length 0 gets zeros. Unless acc is NULL, the token's weights are added to
+ * it as ming_cuda_attn_weights does (the token's own entry is set). q_start,
+ * rows and max_rows are not used; lse is NULL. */
+int ming_cuda_attn_decode(ming_ctx* ctx, const ming_kv_cache* cache, const ming_attn* attn);
+
+/* Eviction: of each (sequence, layer, kv head) of `from` that holds more
+ * than `keep` positions, the first `sinks`, the last `recent` and, of those
+ * between, the keep - sinks - recent of the largest total in acc stay (ties:
+ * the lowest positions; NaN counts as -infinity); a sequence of at most
+ * `keep` positions stays whole. What stays moves, in order, to positions
+ * 0, 1, .. of `to` (keys as they are: rotated for their first positions),
+ * its totals to acc_to. index, unless NULL, receives the positions that
+ * stayed, [seqs][layers][kv_heads][keep], -1 behind them. Each sequence then
+ * holds min(len, keep) positions; lens is not written and to's is not read.
+ * `to` may be `from` with acc_to = acc (in place); else the pages and totals
+ * of the two do not overlap. A page shared by two sequences must not be
+ * evicted in place. acc and acc_to may be NULL if keep = sinks + recent. */
+typedef struct ming_evict {
+    int keep, sinks, recent;
+    const float* acc;
+    int64_t acc_seq_stride, acc_layer_stride, acc_head_stride;
+    float* acc_to;
+    int64_t acc_to_seq_stride, acc_to_layer_stride, acc_to_head_stride;
+    int* index;
+    void* stream;
+} ming_evict;
+int ming_cuda_kv_evict(ming_ctx* ctx, const ming_kv_cache* from, const ming_kv_cache* to, const ming_evict* evict);
+
 /* The context's CUDA stream (a cudaStream_t), for event timing by callers. */
 int ming_cuda_get_stream(ming_ctx* ctx, void** stream);
 int ming_cuda_sync(ming_ctx* ctx);

@@ -1,0 +1,107 @@
+// attn.cuh — attention over bounded paged K/V caches and their eviction:
+// what the operators' kernels share (attn_decode.cu: one new token per
+// sequence; attn_prefill.cu: a prompt's rows, and the weights they gave;
+// kv_evict.cu: eviction by accumulated weight), and their launchers. The
+// host side (argument checks, the C entry points) is attn_api.cu.
+//
+// Row i of a sequence holding len positions, n of them the rows' own, sits at
+// position p = len - n + i and sees j <= p with j < sinks or j > p - window
+// (window 0: every j <= p). s_ij = scale q_i . k_j, summed in f32 over exact
+// bf16 products; out_i = sum_j exp(s_ij - lse_i) v_j, rounded to bf16 once.
+#pragma once
+
+#include "common.cuh"
+
+namespace ming {
+
+constexpr int AT_PAGE = 16;     // positions per page
+constexpr int AT_HD = 64;       // head dim
+constexpr int AT_MAXG = 8;      // query heads per kv head
+constexpr float AT_LOG2E = 1.4426950408889634f;
+
+// Device error codes (the context's error word, read by ming_cuda_sync)
+constexpr int AT_ERR_PAGE = 16;  // a block table entry outside the pool (page 0 was read instead, nothing written)
+constexpr int AT_ERR_LEN = 17;   // a length outside [0, max_len] (clamped)
+constexpr int AT_ERR_ROWS = 18;  // q_start is not ascending within [0, rows], or a sequence has more than max_rows rows (clamped)
+constexpr int AT_ERR_WAIT = 19;  // a bounded device wait expired
+
+// A paged cache: element (page, layer, kv head, slot, dim) of K at
+// k[page * ps + layer * ls + head * hs + slot * ss + dim].
+struct KvPages {
+    uint16_t *k, *v;
+    int64_t ps, hs, ss;
+    const int* bt;       // [seqs][bt_ld]
+    const int* lens;     // [seqs]
+    const int* seq_ids;  // row b of the batch is sequence seq_ids[b] of bt, lens and acc (null: b)
+    int bt_ld, pages, max_len;
+    int len_add;         // positions to add to lens (the model's step: its own position is not counted yet)
+};
+
+struct AttnOp {
+    KvPages kv;          // k, v already at the layer
+    const uint16_t* q;
+    uint16_t* out;
+    int64_t q_rs, q_hs, o_rs, o_hs;  // element strides of rows and heads
+    const int* q_start;  // [seqs + 1] or null (decode: row b)
+    float* lse;          // [rows][heads]
+    float* acc;          // + seq * a_ss + kv head * a_hs + j
+    int64_t a_ss, a_hs;
+    int seqs, rows, max_rows, heads, kv_heads, group, window, sinks;
+    float scale_log2;    // scale * log2(e)
+    int* err;
+};
+
+struct EvictOp {
+    KvPages from, to;    // k, v at layer 0
+    int64_t from_ls, to_ls;
+    const float* acc;
+    float* acc_to;
+    int64_t a_ss, a_ls, a_hs, t_ss, t_ls, t_hs;
+    int* index;          // [seqs][layers][kv_heads][keep] or null
+    int seqs, layers, kv_heads, keep, sinks, recent;
+    int* err;
+};
+
+cudaError_t launch_attn_prefill(const AttnOp& a, cudaStream_t s);
+cudaError_t launch_attn_weights(const AttnOp& a, cudaStream_t s);
+cudaError_t launch_attn_decode(const AttnOp& a, cudaStream_t s);
+cudaError_t launch_kv_evict(const EvictOp& a, cudaStream_t s);
+
+MING_DEV void at_flag(int* err, int code) {
+    if (err) atomicCAS(err, 0, code);
+}
+MING_DEV int at_seq(const KvPages& kv, int b) { return kv.seq_ids ? kv.seq_ids[b] : b; }
+// The sequence's positions, clamped into [0, max_len].
+MING_DEV int at_len(const KvPages& kv, int seq, int* err) {
+    const int n = kv.lens[seq] + kv.len_add;
+    if (n < 0 || n > kv.max_len) {
+        at_flag(err, AT_ERR_LEN);
+        return n < 0 ? 0 : kv.max_len;
+    }
+    return n;
+}
+// The page that holds page-index i of a sequence's table row, 0 if the entry
+// lies outside the pool.
+MING_DEV int at_page(const KvPages& kv, const int* row, int i, int* err) {
+    const int p = row[i];
+    if ((unsigned)p < (unsigned)kv.pages) return p;
+    at_flag(err, AT_ERR_PAGE);
+    return 0;
+}
+// A sequence's rows [r0, r1) of q, clamped into [0, rows] and to max_rows.
+MING_DEV void at_rows(const AttnOp& a, int b, int& r0, int& r1) {
+    r0 = a.q_start[b];
+    r1 = a.q_start[b + 1];
+    if (r0 < 0 || r1 > a.rows || r1 < r0 || r1 - r0 > a.max_rows) {
+        at_flag(a.err, AT_ERR_ROWS);
+        r0 = min(max(r0, 0), a.rows);
+        r1 = min(max(r1, r0), min(a.rows, r0 + a.max_rows));
+    }
+}
+// What a row at position p sees: [0, s1) and [w0, p], s1 <= w0.
+MING_DEV void at_sees(int p, int window, int sinks, int& s1, int& w0) {
+    w0 = window ? max(0, p + 1 - window) : 0;
+    s1 = min(sinks, w0);
+}
+
+}  // namespace ming

@@ -1,0 +1,216 @@
+// attn_api.cu — the C entry points of the operators on caller-owned paged
+// caches (include/ming_cuda.h): argument checks on the host, then one launch.
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <string>
+
+#include "attn.cuh"
+#include "runtime.h"
+
+using namespace ming;
+using namespace ming::rt;
+
+namespace {
+
+// Makes the context's device current and puts the caller's back.
+struct OnDevice {
+    int prev = -1;
+    cudaError_t e;
+    explicit OnDevice(int device) {
+        e = cudaGetDevice(&prev);
+        if (e == cudaSuccess && prev != device) e = cudaSetDevice(device);
+        else prev = -1;
+    }
+    ~OnDevice() {
+        if (prev >= 0) cudaSetDevice(prev);
+    }
+};
+
+bool misaligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
+
+int check_cache(const ming_kv_cache* c, const char* name) {
+    const std::string s(name);
+    if (!c) return fail(MING_ERR_INVALID, s + " is null");
+    if (!c->k || !c->v || (c->seqs && (!c->block_table || !c->lens))) return fail(MING_ERR_INVALID, s + ": null pointer");
+    if (misaligned(c->k, 16) || misaligned(c->v, 16)) return fail(MING_ERR_INVALID, s + ": k and v must be 16-byte aligned");
+    if (misaligned(c->block_table, 4) || misaligned(c->lens, 4))
+        return fail(MING_ERR_INVALID, s + ": block_table and lens must be 4-byte aligned");
+    if (c->pages < 1 || c->layers < 1 || c->kv_heads < 1 || c->seqs < 0 || c->bt_ld < 1)
+        return fail(MING_ERR_INVALID, s + ": bad pages, layers, kv_heads, seqs or bt_ld");
+    if (c->seqs > 65535 || c->kv_heads > 65535 || c->layers > 65535)
+        return fail(MING_ERR_INVALID, s + ": at most 65535 sequences, layers and kv heads");
+    if (c->page_stride % 8 || c->layer_stride % 8 || c->head_stride % 8 || c->slot_stride % 8)
+        return fail(MING_ERR_INVALID, s + ": strides must be multiples of 8 elements");
+    if (c->page_stride < 0 || c->layer_stride < 0 || c->head_stride < 0 || c->slot_stride < 0)
+        return fail(MING_ERR_INVALID, s + ": negative stride");
+    if (c->slot_stride < AT_HD) return fail(MING_ERR_INVALID, s + ": slot_stride is below the head dim");
+    if (c->max_len < 0 || (int64_t)c->max_len > (int64_t)c->bt_ld * AT_PAGE)
+        return fail(MING_ERR_INVALID, s + ": max_len does not fit the block table");
+    return MING_OK;
+}
+
+KvPages pages_of(const ming_kv_cache* c, int layer) {
+    KvPages p{};
+    p.k = c->k + layer * c->layer_stride;
+    p.v = c->v + layer * c->layer_stride;
+    p.ps = c->page_stride;
+    p.hs = c->head_stride;
+    p.ss = c->slot_stride;
+    p.bt = c->block_table;
+    p.lens = c->lens;
+    p.bt_ld = c->bt_ld;
+    p.pages = c->pages;
+    p.max_len = c->max_len;
+    return p;
+}
+
+// Checks what the attention operators share and fills the kernels' argument.
+int attn_op(ming_ctx* c, const ming_kv_cache* kv, const ming_attn* f, bool prompt, AttnOp* a) {
+    int rc = check_cache(kv, "cache");
+    if (rc) return rc;
+    if (!f) return fail(MING_ERR_INVALID, "attn is null");
+    if (f->heads < 1 || f->heads > 65535 || f->heads % kv->kv_heads || f->heads / kv->kv_heads > AT_MAXG)
+        return fail(MING_ERR_INVALID, "heads must be a multiple of the cache's kv_heads with at most 8 per group");
+    if (f->layer < 0 || f->layer >= kv->layers) return fail(MING_ERR_INVALID, "layer out of range");
+    if (f->window < 0 || f->sinks < 0) return fail(MING_ERR_INVALID, "window and sinks must not be negative");
+    if (!(f->scale >= 0.f) || std::isinf(f->scale)) return fail(MING_ERR_INVALID, "scale must be finite and not negative");
+    const bool rows = prompt ? f->rows != 0 : kv->seqs != 0;  // without any, q, out and lse may be null
+    if (!f->q && rows) return fail(MING_ERR_INVALID, "q is null");
+    if (misaligned(f->q, 16) || f->q_row_stride % 8 || f->q_head_stride % 8 || f->q_row_stride < 0 || f->q_head_stride < 0)
+        return fail(MING_ERR_INVALID, "q must be 16-byte aligned, its strides multiples of 8 elements and not negative");
+    if (prompt) {
+        if (!f->q_start) return fail(MING_ERR_INVALID, "q_start is null");
+        if (misaligned(f->q_start, 4)) return fail(MING_ERR_INVALID, "q_start must be 4-byte aligned");
+        if (f->rows < 0 || f->max_rows < 0 || f->max_rows > f->rows)
+            return fail(MING_ERR_INVALID, "rows and max_rows must satisfy 0 <= max_rows <= rows");
+    }
+    if (misaligned(f->lse, 4) || misaligned(f->acc, 4)) return fail(MING_ERR_INVALID, "lse and acc must be 4-byte aligned");
+    if (f->acc && (f->acc_seq_stride < 0 || f->acc_layer_stride < 0 || f->acc_head_stride < 0))
+        return fail(MING_ERR_INVALID, "acc: negative stride");
+    *a = AttnOp{};
+    a->kv = pages_of(kv, f->layer);
+    a->q = f->q;
+    a->out = f->out;
+    a->q_rs = f->q_row_stride;
+    a->q_hs = f->q_head_stride;
+    a->o_rs = f->out_row_stride;
+    a->o_hs = f->out_head_stride;
+    a->q_start = prompt ? f->q_start : nullptr;
+    a->lse = f->lse;
+    a->acc = f->acc ? f->acc + f->layer * f->acc_layer_stride : nullptr;
+    a->a_ss = f->acc_seq_stride;
+    a->a_hs = f->acc_head_stride;
+    a->seqs = kv->seqs;
+    a->rows = prompt ? f->rows : kv->seqs;
+    a->max_rows = prompt ? f->max_rows : 1;
+    a->heads = f->heads;
+    a->kv_heads = kv->kv_heads;
+    a->group = f->heads / kv->kv_heads;
+    a->window = f->window;
+    a->sinks = f->sinks;
+    a->scale_log2 = (f->scale == 0.f ? 0.125f : f->scale) * AT_LOG2E;
+    a->err = c ? c->dev_err : nullptr;
+    return MING_OK;
+}
+
+int check_out(const ming_attn* f, bool rows) {
+    if (!f->out && rows) return fail(MING_ERR_INVALID, "out is null");
+    if (misaligned(f->out, 16) || f->out_row_stride % 8 || f->out_head_stride % 8 || f->out_row_stride < 0 ||
+        f->out_head_stride < 0)
+        return fail(MING_ERR_INVALID, "out must be 16-byte aligned, its strides multiples of 8 elements and not negative");
+    return MING_OK;
+}
+
+// The arguments are checked before the context: a refusal names what is wrong
+// with the call.
+template <class Op>
+int launch(ming_ctx* c, void* stream, const char* name, cudaError_t (*go)(const Op&, cudaStream_t), const Op& a, bool empty) {
+    if (!c) return fail(MING_ERR_INVALID, "null context");
+    if (empty) return MING_OK;
+    OnDevice dev(c->device);
+    if (dev.e != cudaSuccess) return fail(MING_ERR_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(dev.e));
+    const cudaError_t e = go(a, stream ? static_cast<cudaStream_t>(stream) : c->stream);
+    if (e != cudaSuccess) return fail(MING_ERR_CUDA, std::string(name) + ": " + cudaGetErrorString(e));
+    return MING_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ming_cuda_attn_prefill(ming_ctx* c, const ming_kv_cache* kv, const ming_attn* f) {
+    AttnOp a;
+    int rc = attn_op(c, kv, f, true, &a);
+    if (rc) return rc;
+    if ((rc = check_out(f, a.rows != 0))) return rc;
+    if (f->acc) return fail(MING_ERR_INVALID, "acc must be null (ming_cuda_attn_weights adds a prompt's weights)");
+    return launch(c, f->stream, "attn_prefill", launch_attn_prefill, a, !a.seqs || !a.max_rows);
+}
+
+int ming_cuda_attn_weights(ming_ctx* c, const ming_kv_cache* kv, const ming_attn* f) {
+    AttnOp a;
+    int rc = attn_op(c, kv, f, true, &a);
+    if (rc) return rc;
+    if (!f->lse && a.rows) return fail(MING_ERR_INVALID, "lse is null");
+    if (!f->acc) return fail(MING_ERR_INVALID, "acc is null");
+    return launch(c, f->stream, "attn_weights", launch_attn_weights, a, !a.seqs || !a.max_rows || !a.kv.max_len);
+}
+
+int ming_cuda_attn_decode(ming_ctx* c, const ming_kv_cache* kv, const ming_attn* f) {
+    AttnOp a;
+    int rc = attn_op(c, kv, f, false, &a);
+    if (rc) return rc;
+    if ((rc = check_out(f, a.rows != 0))) return rc;
+    if (f->lse) return fail(MING_ERR_INVALID, "lse must be null");
+    return launch(c, f->stream, "attn_decode", launch_attn_decode, a, !a.seqs);
+}
+
+int ming_cuda_kv_evict(ming_ctx* c, const ming_kv_cache* from, const ming_kv_cache* to, const ming_evict* f) {
+    int rc = check_cache(from, "from");
+    if (rc) return rc;
+    if ((rc = check_cache(to, "to"))) return rc;
+    if (!f) return fail(MING_ERR_INVALID, "evict is null");
+    if (to->layers != from->layers || to->kv_heads != from->kv_heads || to->seqs != from->seqs)
+        return fail(MING_ERR_INVALID, "from and to differ in layers, kv_heads or seqs");
+    if (f->sinks < 0 || f->recent < 0 || f->keep < 1 || (int64_t)f->sinks + f->recent > f->keep)
+        return fail(MING_ERR_INVALID, "sinks and recent must not be negative and fit in keep, which is at least 1");
+    if ((int64_t)(f->keep < from->max_len ? f->keep : from->max_len) > (int64_t)to->bt_ld * AT_PAGE)
+        return fail(MING_ERR_INVALID, "what stays does not fit to's block table");
+    if (!f->acc && f->sinks + f->recent != f->keep)
+        return fail(MING_ERR_INVALID, "acc is null: keep must be sinks + recent");
+    if ((f->acc != nullptr) != (f->acc_to != nullptr)) return fail(MING_ERR_INVALID, "acc and acc_to go together");
+    if (misaligned(f->acc, 4) || misaligned(f->acc_to, 4) || misaligned(f->index, 4))
+        return fail(MING_ERR_INVALID, "acc, acc_to and index must be 4-byte aligned");
+    if (f->acc && (f->acc_seq_stride < 0 || f->acc_layer_stride < 0 || f->acc_head_stride < 0 || f->acc_to_seq_stride < 0 ||
+                   f->acc_to_layer_stride < 0 || f->acc_to_head_stride < 0))
+        return fail(MING_ERR_INVALID, "acc: negative stride");
+    if (f->acc == f->acc_to && f->acc &&
+        (f->acc_seq_stride != f->acc_to_seq_stride || f->acc_layer_stride != f->acc_to_layer_stride ||
+         f->acc_head_stride != f->acc_to_head_stride))
+        return fail(MING_ERR_INVALID, "acc and acc_to are the same buffer with other strides");
+    EvictOp a{};
+    a.from = pages_of(from, 0);
+    a.to = pages_of(to, 0);
+    a.from_ls = from->layer_stride;
+    a.to_ls = to->layer_stride;
+    a.acc = f->acc;
+    a.acc_to = f->acc_to;
+    a.a_ss = f->acc_seq_stride;
+    a.a_ls = f->acc_layer_stride;
+    a.a_hs = f->acc_head_stride;
+    a.t_ss = f->acc_to_seq_stride;
+    a.t_ls = f->acc_to_layer_stride;
+    a.t_hs = f->acc_to_head_stride;
+    a.index = f->index;
+    a.seqs = from->seqs;
+    a.layers = from->layers;
+    a.kv_heads = from->kv_heads;
+    a.keep = f->keep;
+    a.sinks = f->sinks;
+    a.recent = f->recent;
+    a.err = c ? c->dev_err : nullptr;
+    return launch(c, f->stream, "kv_evict", launch_kv_evict, a, !a.seqs);
+}
+
+}  // extern "C"

@@ -15,6 +15,7 @@
 #include <vector>
 
 #include "runtime.h"
+#include "attn.cuh"
 #include "dispatch.cuh"
 #include "bulk.cuh"
 #include "dit.cuh"
@@ -543,7 +544,6 @@ int setup_mega(ming_ctx* c) {
     unsigned long long* acc = c->mem.alloc<unsigned long long>(acc_n, &rc);
     const size_t hbuf_n = (size_t)f.layers * MG_MAXB * f.ff;
     uint64_t* hbuf = c->mem.alloc<uint64_t>(hbuf_n, &rc);
-    c->dev_err = c->mem.alloc<int>(1, &rc);
     c->mega_counter = c->mem.alloc<int>(2, &rc);
     if (rc) return rc;
     int* counter = c->mega_counter;
@@ -622,9 +622,13 @@ int check_dev_err(ming_ctx* c) {
     if (e) {
         const int zero = 0;
         cudaMemcpy(c->dev_err, &zero, 4, cudaMemcpyHostToDevice);
+        if (e == AT_ERR_PAGE) return fail(MING_ERR_CUDA, "a block table entry lies outside the page pool");
+        if (e == AT_ERR_LEN) return fail(MING_ERR_CUDA, "a sequence's length lies outside [0, max_len]");
+        if (e == AT_ERR_ROWS) return fail(MING_ERR_CUDA, "q_start does not describe at most max_rows rows per sequence within rows");
         if (c->mega_reset) c->mega_reset();
         return fail(MING_ERR_CUDA, std::string(e == BK_ERR_WEIGHTS   ? "decode-batch linear: weight copy"
                                                : e == ATT_ERR_PAGES ? "attention: K/V page copy"
+                                               : e == AT_ERR_WAIT   ? "attention over a paged cache"
                                                                     : "persistent decode kernel") +
                                        ": a bounded device wait expired (code " + std::to_string(e) + ")");
     }
@@ -856,6 +860,9 @@ int ming_cuda_create(int device, const ming_cfg* cfg, ming_ctx** out) {
     c->device = device;
     c->cfg = f;
     CK(cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking));
+    int rc = MING_OK;
+    c->dev_err = c->mem.alloc<int>(1, &rc);
+    if (rc) return rc;
     *out = c.release();
     return MING_OK;
 }
@@ -1079,8 +1086,6 @@ int ming_cuda_finalize(ming_ctx* c) {
         c->lin.rows = rows_cap;
         c->lin.K = k_cap;
         CK(cudaDeviceGetAttribute(&c->lin.sms, cudaDevAttrMultiProcessorCount, c->device));
-        if (!c->dev_err) c->dev_err = c->mem.alloc<int>(1, &rc);
-        if (rc) return rc;
         if (!c->err_host && cudaHostAlloc(reinterpret_cast<void**>(&c->err_host), 4, cudaHostAllocDefault) != cudaSuccess) {
             cudaGetLastError();
             c->err_host = nullptr;  // the error flag is then read with a synchronous copy

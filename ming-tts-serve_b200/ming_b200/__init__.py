@@ -35,6 +35,7 @@ SYMBOLS = [
     "ming_cuda_default_sample_params", "ming_cuda_sample_latents", "ming_cuda_loop_create", "ming_cuda_loop_submit",
     "ming_cuda_loop_step", "ming_cuda_loop_result", "ming_cuda_loop_destroy", "ming_cuda_load_safetensors",
     "ming_cuda_vae_decode",
+    "ming_cuda_attn_prefill", "ming_cuda_attn_weights", "ming_cuda_attn_decode", "ming_cuda_kv_evict",
 ]
 
 
@@ -52,6 +53,35 @@ class SampleParams(ctypes.Structure):
     """ming_sample_params: SampleParams (src/ming_model.zig:1368-1373) + max_len."""
     _fields_ = [("max_steps", ctypes.c_int), ("max_len", ctypes.c_int), ("cfg", ctypes.c_float),
                 ("sigma", ctypes.c_float), ("temperature", ctypes.c_float)]
+
+
+class KvCacheArgs(ctypes.Structure):
+    """ming_kv_cache."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("page_stride", ctypes.c_int64),
+                ("layer_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("slot_stride", ctypes.c_int64),
+                ("pages", ctypes.c_int), ("layers", ctypes.c_int), ("kv_heads", ctypes.c_int), ("seqs", ctypes.c_int),
+                ("block_table", ctypes.c_void_p), ("bt_ld", ctypes.c_int), ("max_len", ctypes.c_int),
+                ("lens", ctypes.c_void_p)]
+
+
+class AttnArgs(ctypes.Structure):
+    """ming_attn."""
+    _fields_ = [("layer", ctypes.c_int), ("heads", ctypes.c_int), ("window", ctypes.c_int), ("sinks", ctypes.c_int),
+                ("scale", ctypes.c_float), ("q", ctypes.c_void_p), ("q_row_stride", ctypes.c_int64),
+                ("q_head_stride", ctypes.c_int64), ("out", ctypes.c_void_p), ("out_row_stride", ctypes.c_int64),
+                ("out_head_stride", ctypes.c_int64), ("q_start", ctypes.c_void_p), ("rows", ctypes.c_int),
+                ("max_rows", ctypes.c_int), ("lse", ctypes.c_void_p), ("acc", ctypes.c_void_p),
+                ("acc_seq_stride", ctypes.c_int64), ("acc_layer_stride", ctypes.c_int64),
+                ("acc_head_stride", ctypes.c_int64), ("stream", ctypes.c_void_p)]
+
+
+class EvictArgs(ctypes.Structure):
+    """ming_evict."""
+    _fields_ = [("keep", ctypes.c_int), ("sinks", ctypes.c_int), ("recent", ctypes.c_int), ("acc", ctypes.c_void_p),
+                ("acc_seq_stride", ctypes.c_int64), ("acc_layer_stride", ctypes.c_int64),
+                ("acc_head_stride", ctypes.c_int64), ("acc_to", ctypes.c_void_p), ("acc_to_seq_stride", ctypes.c_int64),
+                ("acc_to_layer_stride", ctypes.c_int64), ("acc_to_head_stride", ctypes.c_int64),
+                ("index", ctypes.c_void_p), ("stream", ctypes.c_void_p)]
 
 
 class MingError(RuntimeError):
@@ -104,6 +134,10 @@ def lib():
         "ming_cuda_loop_destroy": (I, [P]),
         "ming_cuda_load_safetensors": (I, [P, ctypes.c_char_p, IP]),
         "ming_cuda_vae_decode": (I, [P, P, I, P, I]),
+        "ming_cuda_attn_prefill": (I, [P, P, P]),
+        "ming_cuda_attn_weights": (I, [P, P, P]),
+        "ming_cuda_attn_decode": (I, [P, P, P]),
+        "ming_cuda_kv_evict": (I, [P, P, P, P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -169,6 +203,68 @@ def _dtype_code(a):
     raise TypeError(f"unsupported dtype {a.dtype}")
 
 
+def _want(ok, what):
+    if not ok:
+        raise MingError(what)
+
+
+def _tensor(t, name, dtype, ndim, device=None):
+    """Checks a device tensor (torch's interface: dtype, dim(), stride(), device)."""
+    _want(hasattr(t, "data_ptr") and hasattr(t, "stride"), f"{name}: a device tensor is wanted")
+    _want(str(t.dtype) == dtype, f"{name}: {dtype} is wanted, got {t.dtype}")
+    _want(t.dim() == ndim, f"{name}: {ndim} dimensions are wanted, got {t.dim()}")
+    _want(t.device.type == "cuda" and (device is None or t.device.index == device), f"{name} is on {t.device}")
+    _want(t.shape[-1] <= 1 or t.stride(-1) == 1, f"{name}: the last dimension must be contiguous")
+
+
+def _strides(t):
+    """Strides with 0 for dimensions of one element, which are never strided over."""
+    return [st if n > 1 else 0 for n, st in zip(t.shape, t.stride())]
+
+
+def _stream(stream):
+    """The C entry points read NULL as the context's stream; the legacy default
+    stream, whose handle is 0 in Python, has the explicit handle 1."""
+    return None if stream is None else (stream or 1)
+
+
+class KvCache:
+    """A paged K/V cache in the caller's device memory (ming_kv_cache).
+
+    k, v: bf16 [pages, layers, kv_heads, 16, 64], views of any layout with the
+    same strides and contiguous dims (the context's own pool is
+    [pages, layers, K|V, kv_heads, 16, 64]); block_table: int32 [seqs, n];
+    lens: int32 [seqs]; max_len: no sequence holds more positions."""
+
+    def __init__(self, k, v, block_table, lens, max_len):
+        bf16, i32 = "torch.bfloat16", "torch.int32"
+        _tensor(k, "k", bf16, 5)
+        self.device = k.device.index
+        _tensor(v, "v", bf16, 5, self.device)
+        _want(k.shape == v.shape and _strides(k) == _strides(v), "k and v differ in shape or strides")
+        _want(k.shape[3] == 16 and k.shape[4] == 64, "k and v: pages of 16 positions and heads of 64 dims are wanted")
+        _tensor(block_table, "block_table", i32, 2, self.device)
+        _tensor(lens, "lens", i32, 1, self.device)
+        _want(lens.shape[0] == block_table.shape[0], "lens and block_table differ in sequences")
+        self.k, self.v, self.block_table, self.lens, self.max_len = k, v, block_table, lens, int(max_len)
+        s = _strides(k)
+        self.args = KvCacheArgs(k.data_ptr(), v.data_ptr(), s[0], s[1], s[2], s[3], k.shape[0], k.shape[1], k.shape[2],
+                                lens.shape[0], block_table.data_ptr(),
+                                block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1],
+                                self.max_len, lens.data_ptr())
+        _want(self.max_len <= 16 * block_table.shape[1], "max_len does not fit the block table")
+        self.ref = ctypes.addressof(self.args)
+
+    def _acc(self, acc, name="acc"):
+        """(address, seq, layer and head stride) of running totals f32 [seqs, layers, kv_heads, >= max_len]."""
+        if acc is None:
+            return None, 0, 0, 0
+        _tensor(acc, name, "torch.float32", 4, self.device)
+        _want(tuple(acc.shape[:3]) == (self.args.seqs, self.args.layers, self.args.kv_heads) and
+              acc.shape[3] >= self.max_len, f"{name}: [seqs, layers, kv_heads, at least max_len] is wanted")
+        return (acc.data_ptr(),) + tuple(_strides(acc)[:3])
+
+
 class Context:
     """One device context (ming_ctx). Mirrors the reference Model's hot-path
     surface: load, lm_prefill/lm_decode (lmForward), generate (the token loop),
@@ -178,6 +274,7 @@ class Context:
         """weights: {name: array} loaded tensor by tensor; checkpoint: a
         safetensors file (or a directory holding model.safetensors)."""
         self.cfg = cfg if cfg is not None else default_cfg()
+        self.device = device
         self._h = ctypes.c_void_p()
         _check(lib().ming_cuda_create(device, ctypes.byref(self.cfg), ctypes.byref(self._h)))
         if checkpoint is not None:
@@ -334,6 +431,79 @@ class Context:
         v = np.ascontiguousarray(v, dtype=np.uint16)
         assert k.shape == v.shape and k.shape[0] == self.cfg.kv_heads and k.shape[2] == 64
         _check(lib().ming_cuda_kv_write(self._h, s, layer, pos0, k.shape[1], _ptr(k), _ptr(v)))
+
+    def _attn(self, q, cache, layer, window, sinks, scale, stream):
+        _tensor(q, "q", "torch.bfloat16", 3, self.device)
+        _want(q.shape[2] == 64, "q: heads of 64 dims are wanted")
+        _want(cache.device == self.device, "the cache is on another device")
+        s = _strides(q)
+        return AttnArgs(layer, q.shape[1], window, sinks, scale or 0.0, q.data_ptr(), s[0], s[1], stream=_stream(stream))
+
+    def _attn_out(self, a, q, out):
+        _tensor(out, "out", "torch.bfloat16", 3, self.device)
+        _want(out.shape == q.shape, "out and q differ in shape")
+        a.out = out.data_ptr()
+        a.out_row_stride, a.out_head_stride = _strides(out)[:2]
+
+    def _attn_rows(self, a, q, q_start, cache, lse, max_rows):
+        _tensor(q_start, "q_start", "torch.int32", 1, self.device)
+        _want(q_start.shape[0] == cache.args.seqs + 1, "q_start: seqs + 1 entries are wanted")
+        a.q_start, a.rows = q_start.data_ptr(), q.shape[0]
+        a.max_rows = q.shape[0] if max_rows is None else max_rows
+        if lse is not None:
+            _tensor(lse, "lse", "torch.float32", 2, self.device)
+            _want(lse.shape == q.shape[:2] and lse.is_contiguous(), "lse: contiguous [rows, heads] is wanted")
+            a.lse = lse.data_ptr()
+
+    def attn_prefill(self, q, q_start, cache, out, lse=None, *, max_rows=None, layer=0, window=0, sinks=0, scale=None,
+                     stream=None):
+        """ming_cuda_attn_prefill: q, out bf16 [rows, heads, 64]; q_start int32
+        [seqs + 1]; cache a KvCache that holds the rows' own keys and values;
+        lse f32 [rows, heads] or None. stream: a CUDA stream's handle (None:
+        the context's stream). Device tensors, asynchronous."""
+        a = self._attn(q, cache, layer, window, sinks, scale, stream)
+        self._attn_out(a, q, out)
+        self._attn_rows(a, q, q_start, cache, lse, max_rows)
+        _check(lib().ming_cuda_attn_prefill(self._h, cache.ref, ctypes.addressof(a)))
+        return out
+
+    def attn_weights(self, q, q_start, cache, lse, acc, *, max_rows=None, layer=0, window=0, sinks=0, scale=None,
+                     stream=None):
+        """ming_cuda_attn_weights: the weights of attn_prefill's rows (its lse)
+        added to acc f32 [seqs, layers, kv_heads, >= max_len]."""
+        a = self._attn(q, cache, layer, window, sinks, scale, stream)
+        self._attn_rows(a, q, q_start, cache, lse, max_rows)
+        a.acc, a.acc_seq_stride, a.acc_layer_stride, a.acc_head_stride = cache._acc(acc)
+        _check(lib().ming_cuda_attn_weights(self._h, cache.ref, ctypes.addressof(a)))
+        return acc
+
+    def attn_decode(self, q, cache, out, acc=None, *, layer=0, window=0, sinks=0, scale=None, stream=None):
+        """ming_cuda_attn_decode: one new token per sequence, q and out bf16
+        [seqs, heads, 64]; its weights are added to acc unless that is None."""
+        a = self._attn(q, cache, layer, window, sinks, scale, stream)
+        _want(q.shape[0] == cache.args.seqs, "q: one row per sequence is wanted")
+        self._attn_out(a, q, out)
+        if acc is not None:
+            a.acc, a.acc_seq_stride, a.acc_layer_stride, a.acc_head_stride = cache._acc(acc)
+        _check(lib().ming_cuda_attn_decode(self._h, cache.ref, ctypes.addressof(a)))
+        return out
+
+    def kv_evict(self, cache, to=None, acc=None, acc_to=None, *, keep, sinks=0, recent=0, index=None, stream=None):
+        """ming_cuda_kv_evict: what stays of every (sequence, layer, kv head)
+        moves to the cache `to` and its totals to acc_to; to None: in place.
+        index: int32 [seqs, layers, kv_heads, keep] or None. The sequences
+        then hold min(len, keep) positions (lens is the caller's to update)."""
+        _want(cache.device == self.device and (to is None or to.device == self.device), "the cache is on another device")
+        if to is None:
+            to, acc_to = cache, acc
+        _want(acc_to is None or acc is not None, "acc_to is given without acc")
+        e = EvictArgs(keep, sinks, recent, *cache._acc(acc), *to._acc(acc_to, "acc_to"), stream=_stream(stream))
+        if index is not None:
+            _tensor(index, "index", "torch.int32", 4, self.device)
+            _want(tuple(index.shape) == (cache.args.seqs, cache.args.layers, cache.args.kv_heads, keep) and
+                  index.is_contiguous(), "index: contiguous [seqs, layers, kv_heads, keep] is wanted")
+            e.index = index.data_ptr()
+        _check(lib().ming_cuda_kv_evict(self._h, cache.ref, to.ref, ctypes.addressof(e)))
 
     def unpack_linear(self, weight_name, out_dim, in_dim):
         out = np.empty((out_dim, in_dim), dtype=np.float32)

@@ -1,0 +1,128 @@
+"""CPU tests of the operators on caller-owned paged caches: what their entry
+points refuse, before any CUDA call. A null context is refused last, so that
+a refusal names what is wrong with the call."""
+import ctypes
+
+import pytest
+
+import ming_b200 as M
+from test_abi import _ensure_built
+
+BUF = (ctypes.c_uint8 * 4096)()
+AT = (ctypes.addressof(BUF) + 255) // 256 * 256  # an aligned address; never dereferenced
+
+
+def cache(**kw):
+    c = M.KvCacheArgs(AT, AT, 2 * 2 * 16 * 64, 2 * 2 * 16 * 64, 16 * 64, 64, 9, 1, 2, 3, AT, 4, 60, AT)
+    for k, v in kw.items():
+        setattr(c, k, v)
+    return c
+
+
+def attn(**kw):
+    a = M.AttnArgs(layer=0, heads=14, window=0, sinks=0, scale=0.0, q=AT, q_row_stride=14 * 64, q_head_stride=64, out=AT,
+                   out_row_stride=14 * 64, out_head_stride=64, q_start=AT, rows=20, max_rows=10)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def evict(**kw):
+    e = M.EvictArgs(keep=32, sinks=4, recent=8, acc=AT, acc_seq_stride=256, acc_layer_stride=256, acc_head_stride=128,
+                    acc_to=AT + 64, acc_to_seq_stride=256, acc_to_layer_stride=256, acc_to_head_stride=128)
+    for k, v in kw.items():
+        setattr(e, k, v)
+    return e
+
+
+def refused(rc, *words):
+    assert rc == 1
+    msg = M.lib().ming_cuda_last_error().decode()
+    assert all(w in msg for w in words), msg
+
+
+def call(name, c, a):
+    _ensure_built()
+    return getattr(M.lib(), "ming_cuda_attn_" + name)(None, ctypes.byref(c) if c else None, ctypes.byref(a) if a else None)
+
+
+OPS = {"prefill": {}, "weights": dict(lse=AT, acc=AT), "decode": {}}
+
+
+@pytest.mark.parametrize("op", OPS)
+def test_good_arguments_reach_the_context_check(op):
+    refused(call(op, cache(), attn(**OPS[op])), "null context")
+    refused(call(op, cache(seqs=0), attn(**OPS[op])), "null context")
+    refused(call(op, cache(max_len=0), attn(**OPS[op], window=5, sinks=3)), "null context")
+
+
+@pytest.mark.parametrize("op", OPS)
+@pytest.mark.parametrize("bad,word", [
+    (dict(k=0), "null pointer"), (dict(v=0), "null pointer"), (dict(block_table=0), "null pointer"),
+    (dict(lens=0), "null pointer"), (dict(k=AT + 8), "16-byte"), (dict(v=AT + 2), "16-byte"),
+    (dict(block_table=AT + 2), "4-byte"), (dict(lens=AT + 1), "4-byte"), (dict(pages=0), "pages"),
+    (dict(layers=0), "layers"), (dict(kv_heads=0), "kv_heads"), (dict(seqs=-1), "seqs"), (dict(seqs=65536), "65535"),
+    (dict(bt_ld=0), "bt_ld"), (dict(page_stride=100), "multiples of 8"), (dict(layer_stride=4), "multiples of 8"),
+    (dict(head_stride=-8), "negative"), (dict(slot_stride=56), "head dim"), (dict(max_len=65), "max_len"),
+    (dict(max_len=-1), "max_len"),
+])
+def test_bad_caches_are_refused(op, bad, word):
+    refused(call(op, cache(**bad), attn(**OPS[op])), "cache", word)
+
+
+@pytest.mark.parametrize("op", OPS)
+@pytest.mark.parametrize("bad,word", [
+    (dict(heads=13), "heads"), (dict(heads=0), "heads"), (dict(heads=18), "heads"), (dict(layer=1), "layer"),
+    (dict(layer=-1), "layer"), (dict(window=-1), "window"), (dict(sinks=-1), "sinks"), (dict(scale=-1.0), "scale"),
+    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(q=0), "q is null"),
+    (dict(q=AT + 4), "q must"), (dict(q_row_stride=4), "q must"), (dict(q_head_stride=-64), "q must"),
+])
+def test_bad_attention_arguments_are_refused(op, bad, word):
+    refused(call(op, cache(), attn(**{**OPS[op], **bad})), word)
+
+
+@pytest.mark.parametrize("op,bad,word", [
+    ("prefill", dict(out=0), "out is null"), ("prefill", dict(out=AT + 8), "out must"),
+    ("prefill", dict(out_row_stride=3), "out must"), ("prefill", dict(acc=AT), "acc must be null"),
+    ("prefill", dict(lse=AT + 2), "4-byte"), ("prefill", dict(q_start=0), "q_start"),
+    ("prefill", dict(q_start=AT + 2), "q_start"), ("prefill", dict(rows=-1), "rows"), ("prefill", dict(max_rows=21), "rows"),
+    ("weights", dict(lse=0), "lse is null"), ("weights", dict(acc=0), "acc is null"),
+    ("weights", dict(acc=AT + 1), "4-byte"), ("weights", dict(acc_head_stride=-1), "acc"),
+    ("decode", dict(out=0), "out is null"), ("decode", dict(lse=AT), "lse must be null"),
+    ("decode", dict(acc=AT + 2), "4-byte"), ("decode", dict(acc=AT, acc_seq_stride=-4), "acc"),
+])
+def test_arguments_of_one_operator(op, bad, word):
+    refused(call(op, cache(), attn(**{**OPS[op], **bad})), word)
+
+
+def test_null_structures():
+    for op in OPS:
+        refused(call(op, None, attn()), "null")
+        refused(call(op, cache(), None), "null")
+    L = M.lib()
+    refused(L.ming_cuda_kv_evict(None, None, ctypes.byref(cache()), ctypes.byref(evict())), "from")
+    refused(L.ming_cuda_kv_evict(None, ctypes.byref(cache()), None, ctypes.byref(evict())), "to")
+    refused(L.ming_cuda_kv_evict(None, ctypes.byref(cache()), ctypes.byref(cache()), None), "null")
+
+
+@pytest.mark.parametrize("to,bad,word", [
+    (dict(), dict(), "null context"), (dict(), dict(acc=0, acc_to=0, sinks=24, recent=8), "null context"),
+    (dict(layers=2), dict(), "differ"), (dict(kv_heads=1), dict(), "differ"), (dict(seqs=2), dict(), "differ"),
+    (dict(), dict(keep=0, sinks=0, recent=0), "keep"), (dict(), dict(sinks=-1), "sinks"), (dict(), dict(recent=-1), "recent"),
+    (dict(), dict(sinks=20, recent=13), "fit in keep"), (dict(), dict(sinks=2**31 - 1, recent=2**31 - 1), "fit in keep"),
+    (dict(bt_ld=1, max_len=16), dict(), "does not fit to's"), (dict(), dict(acc=0, acc_to=0), "acc is null"),
+    (dict(), dict(acc_to=0), "go together"), (dict(), dict(acc=0, sinks=24), "go together"), (dict(), dict(index=AT + 2), "4-byte"),
+    (dict(), dict(acc_to_seq_stride=-1), "negative"), (dict(), dict(acc_to=AT, acc_to_head_stride=64), "other strides"),
+])
+def test_evict_arguments(to, bad, word):
+    _ensure_built()
+    refused(M.lib().ming_cuda_kv_evict(None, ctypes.byref(cache()), ctypes.byref(cache(**to)), ctypes.byref(evict(**bad))), word)
+
+
+def test_python_checks():
+    torch = pytest.importorskip("torch")
+    k = torch.zeros(4, 1, 2, 16, 64, dtype=torch.bfloat16)
+    bt, lens = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    for bad in (k.float(), k[0], k):  # another type, too few dimensions, not on a GPU
+        with pytest.raises(M.MingError):
+            M.KvCache(bad, bad, bt, lens, 16)
