@@ -8,6 +8,7 @@ raises if the CUDA library is missing or fails.
 """
 import ctypes
 import os
+import struct
 
 import numpy as np
 
@@ -208,24 +209,31 @@ def _want(ok, what):
         raise MingError(what)
 
 
-def _tensor(t, name, dtype, ndim, device=None):
-    """Checks a device tensor (torch's interface: dtype, dim(), stride(), device)."""
-    _want(hasattr(t, "data_ptr") and hasattr(t, "stride"), f"{name}: a device tensor is wanted")
-    _want(str(t.dtype) == dtype, f"{name}: {dtype} is wanted, got {t.dtype}")
-    _want(t.dim() == ndim, f"{name}: {ndim} dimensions are wanted, got {t.dim()}")
-    _want(t.device.type == "cuda" and (device is None or t.device.index == device), f"{name} is on {t.device}")
-    _want(t.shape[-1] <= 1 or t.stride(-1) == 1, f"{name}: the last dimension must be contiguous")
+_torch_types = None
 
 
-def _strides(t):
-    """Strides with 0 for dimensions of one element, which are never strided over."""
-    return [st if n > 1 else 0 for n, st in zip(t.shape, t.stride())]
+def _types():
+    """torch's bfloat16, float32 and int32 (torch is loaded by the caller, whose tensors these are)."""
+    global _torch_types
+    if _torch_types is None:
+        import torch
+        _torch_types = torch.bfloat16, torch.float32, torch.int32
+    return _torch_types
 
 
-def _stream(stream):
-    """The C entry points read NULL as the context's stream; the legacy default
-    stream, whose handle is 0 in Python, has the explicit handle 1."""
-    return None if stream is None else (stream or 1)
+def _tensor(t, name, dtype, ndim, device):
+    """Checks a device tensor; returns its strides, 0 for dimensions of one
+    element, which are never strided over."""
+    if not hasattr(t, "get_device"):
+        raise MingError(f"{name}: a device tensor is wanted")
+    if t.dtype is not dtype or t.dim() != ndim:
+        raise MingError(f"{name}: {dtype} of {ndim} dimensions is wanted, got {t.dtype} of {t.dim()}")
+    if t.get_device() != device or device < 0:
+        raise MingError(f"{name}: a tensor on cuda:{max(device, 0)} is wanted, it is on {t.device}")
+    s, n = t.stride(), t.shape
+    if s[-1] != 1 and n[-1] > 1:
+        raise MingError(f"{name}: the last dimension must be contiguous")
+    return [0 if k == 1 else x for k, x in zip(n, s)] if 1 in n else s
 
 
 class KvCache:
@@ -237,32 +245,38 @@ class KvCache:
     lens: int32 [seqs]; max_len: no sequence holds more positions."""
 
     def __init__(self, k, v, block_table, lens, max_len):
-        bf16, i32 = "torch.bfloat16", "torch.int32"
-        _tensor(k, "k", bf16, 5)
-        self.device = k.device.index
-        _tensor(v, "v", bf16, 5, self.device)
-        _want(k.shape == v.shape and _strides(k) == _strides(v), "k and v differ in shape or strides")
+        bf16, _, i32 = _types()
+        self.device = k.get_device() if hasattr(k, "get_device") else -1
+        s = _tensor(k, "k", bf16, 5, self.device)
+        _want(list(s) == list(_tensor(v, "v", bf16, 5, self.device)) and k.shape == v.shape, "k and v differ in shape or strides")
         _want(k.shape[3] == 16 and k.shape[4] == 64, "k and v: pages of 16 positions and heads of 64 dims are wanted")
-        _tensor(block_table, "block_table", i32, 2, self.device)
+        st = _tensor(block_table, "block_table", i32, 2, self.device)
         _tensor(lens, "lens", i32, 1, self.device)
         _want(lens.shape[0] == block_table.shape[0], "lens and block_table differ in sequences")
         self.k, self.v, self.block_table, self.lens, self.max_len = k, v, block_table, lens, int(max_len)
-        s = _strides(k)
+        self.seqs, self.shape = lens.shape[0], (lens.shape[0], k.shape[1], k.shape[2])
+        _want(0 <= self.max_len <= 16 * block_table.shape[1], "max_len does not fit the block table")
         self.args = KvCacheArgs(k.data_ptr(), v.data_ptr(), s[0], s[1], s[2], s[3], k.shape[0], k.shape[1], k.shape[2],
-                                lens.shape[0], block_table.data_ptr(),
-                                block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1],
-                                self.max_len, lens.data_ptr())
-        _want(self.max_len <= 16 * block_table.shape[1], "max_len does not fit the block table")
+                                self.seqs, block_table.data_ptr(), st[0] or block_table.shape[1], self.max_len,
+                                lens.data_ptr())
         self.ref = ctypes.addressof(self.args)
 
     def _acc(self, acc, name="acc"):
         """(address, seq, layer and head stride) of running totals f32 [seqs, layers, kv_heads, >= max_len]."""
         if acc is None:
-            return None, 0, 0, 0
-        _tensor(acc, name, "torch.float32", 4, self.device)
-        _want(tuple(acc.shape[:3]) == (self.args.seqs, self.args.layers, self.args.kv_heads) and
-              acc.shape[3] >= self.max_len, f"{name}: [seqs, layers, kv_heads, at least max_len] is wanted")
-        return (acc.data_ptr(),) + tuple(_strides(acc)[:3])
+            return 0, 0, 0, 0
+        s = _tensor(acc, name, _types()[1], 4, self.device)
+        n = acc.shape
+        if n[:3] != self.shape or n[3] < self.max_len:
+            raise MingError(f"{name}: [seqs, layers, kv_heads, at least max_len] is wanted")
+        return acc.data_ptr(), s[0], s[1], s[2]
+
+
+# ming_attn and ming_evict, packed in one step (a structure's fields set one by
+# one take longer than a small launch)
+_ATTN = struct.Struct("@4if P2q P2q P2i P P3q P")
+_EVICT = struct.Struct("@3i P3q P3q P P")
+assert _ATTN.size == ctypes.sizeof(AttnArgs) and _EVICT.size == ctypes.sizeof(EvictArgs)
 
 
 class Context:
@@ -275,6 +289,9 @@ class Context:
         safetensors file (or a directory holding model.safetensors)."""
         self.cfg = cfg if cfg is not None else default_cfg()
         self.device = device
+        # the argument structure of the operators' calls (one thread calls a context)
+        self._args = ctypes.create_string_buffer(max(_ATTN.size, _EVICT.size))
+        self._args_at = ctypes.addressof(self._args)
         self._h = ctypes.c_void_p()
         _check(lib().ming_cuda_create(device, ctypes.byref(self.cfg), ctypes.byref(self._h)))
         if checkpoint is not None:
@@ -432,60 +449,62 @@ class Context:
         assert k.shape == v.shape and k.shape[0] == self.cfg.kv_heads and k.shape[2] == 64
         _check(lib().ming_cuda_kv_write(self._h, s, layer, pos0, k.shape[1], _ptr(k), _ptr(v)))
 
-    def _attn(self, q, cache, layer, window, sinks, scale, stream):
-        _tensor(q, "q", "torch.bfloat16", 3, self.device)
-        _want(q.shape[2] == 64, "q: heads of 64 dims are wanted")
-        _want(cache.device == self.device, "the cache is on another device")
-        s = _strides(q)
-        return AttnArgs(layer, q.shape[1], window, sinks, scale or 0.0, q.data_ptr(), s[0], s[1], stream=_stream(stream))
-
-    def _attn_out(self, a, q, out):
-        _tensor(out, "out", "torch.bfloat16", 3, self.device)
-        _want(out.shape == q.shape, "out and q differ in shape")
-        a.out = out.data_ptr()
-        a.out_row_stride, a.out_head_stride = _strides(out)[:2]
-
-    def _attn_rows(self, a, q, q_start, cache, lse, max_rows):
-        _tensor(q_start, "q_start", "torch.int32", 1, self.device)
-        _want(q_start.shape[0] == cache.args.seqs + 1, "q_start: seqs + 1 entries are wanted")
-        a.q_start, a.rows = q_start.data_ptr(), q.shape[0]
-        a.max_rows = q.shape[0] if max_rows is None else max_rows
+    def _attn(self, call, q, cache, out, q_start, max_rows, lse, acc, layer, window, sinks, scale, stream):
+        bf16, f32, i32 = _types()
+        if cache.device != self.device:
+            raise MingError("the cache is on another device")
+        qs = _tensor(q, "q", bf16, 3, self.device)
+        n = q.shape
+        if n[2] != 64:
+            raise MingError("q: heads of 64 dims are wanted")
+        o, os = 0, (0, 0)
+        if out is not None:
+            os = _tensor(out, "out", bf16, 3, self.device)
+            if out.shape != n:
+                raise MingError("out and q differ in shape")
+            o = out.data_ptr()
+        start = z = 0
+        if q_start is None:
+            if n[0] != cache.seqs:
+                raise MingError("q: one row per sequence is wanted")
+        else:
+            _tensor(q_start, "q_start", i32, 1, self.device)
+            if q_start.shape[0] != cache.seqs + 1:
+                raise MingError("q_start: seqs + 1 entries are wanted")
+            start = q_start.data_ptr()
         if lse is not None:
-            _tensor(lse, "lse", "torch.float32", 2, self.device)
-            _want(lse.shape == q.shape[:2] and lse.is_contiguous(), "lse: contiguous [rows, heads] is wanted")
-            a.lse = lse.data_ptr()
+            _tensor(lse, "lse", f32, 2, self.device)
+            if lse.shape != n[:2] or not lse.is_contiguous():
+                raise MingError("lse: contiguous [rows, heads] is wanted")
+            z = lse.data_ptr()
+        _ATTN.pack_into(self._args, 0, layer, n[1], window, sinks, scale or 0.0, q.data_ptr(), qs[0], qs[1], o, os[0], os[1],
+                        start, n[0], n[0] if max_rows is None else max_rows, z, *cache._acc(acc),
+                        0 if stream is None else stream or 1)
+        _check(call(self._h, cache.ref, self._args_at))
 
     def attn_prefill(self, q, q_start, cache, out, lse=None, *, max_rows=None, layer=0, window=0, sinks=0, scale=None,
                      stream=None):
         """ming_cuda_attn_prefill: q, out bf16 [rows, heads, 64]; q_start int32
         [seqs + 1]; cache a KvCache that holds the rows' own keys and values;
-        lse f32 [rows, heads] or None. stream: a CUDA stream's handle (None:
-        the context's stream). Device tensors, asynchronous."""
-        a = self._attn(q, cache, layer, window, sinks, scale, stream)
-        self._attn_out(a, q, out)
-        self._attn_rows(a, q, q_start, cache, lse, max_rows)
-        _check(lib().ming_cuda_attn_prefill(self._h, cache.ref, ctypes.addressof(a)))
+        lse f32 [rows, heads] or None; max_rows: rows of the sequence with the
+        most. stream: a CUDA stream's handle (0: the legacy default stream,
+        None: the context's stream). Device tensors, asynchronous."""
+        _want(q_start is not None and out is not None, "q_start and out are wanted")
+        self._attn(lib().ming_cuda_attn_prefill, q, cache, out, q_start, max_rows, lse, None, layer, window, sinks, scale, stream)
         return out
 
     def attn_weights(self, q, q_start, cache, lse, acc, *, max_rows=None, layer=0, window=0, sinks=0, scale=None,
                      stream=None):
         """ming_cuda_attn_weights: the weights of attn_prefill's rows (its lse)
         added to acc f32 [seqs, layers, kv_heads, >= max_len]."""
-        a = self._attn(q, cache, layer, window, sinks, scale, stream)
-        self._attn_rows(a, q, q_start, cache, lse, max_rows)
-        a.acc, a.acc_seq_stride, a.acc_layer_stride, a.acc_head_stride = cache._acc(acc)
-        _check(lib().ming_cuda_attn_weights(self._h, cache.ref, ctypes.addressof(a)))
+        _want(q_start is not None, "q_start is wanted")
+        self._attn(lib().ming_cuda_attn_weights, q, cache, None, q_start, max_rows, lse, acc, layer, window, sinks, scale, stream)
         return acc
 
     def attn_decode(self, q, cache, out, acc=None, *, layer=0, window=0, sinks=0, scale=None, stream=None):
         """ming_cuda_attn_decode: one new token per sequence, q and out bf16
         [seqs, heads, 64]; its weights are added to acc unless that is None."""
-        a = self._attn(q, cache, layer, window, sinks, scale, stream)
-        _want(q.shape[0] == cache.args.seqs, "q: one row per sequence is wanted")
-        self._attn_out(a, q, out)
-        if acc is not None:
-            a.acc, a.acc_seq_stride, a.acc_layer_stride, a.acc_head_stride = cache._acc(acc)
-        _check(lib().ming_cuda_attn_decode(self._h, cache.ref, ctypes.addressof(a)))
+        self._attn(lib().ming_cuda_attn_decode, q, cache, out, None, None, None, acc, layer, window, sinks, scale, stream)
         return out
 
     def kv_evict(self, cache, to=None, acc=None, acc_to=None, *, keep, sinks=0, recent=0, index=None, stream=None):
@@ -493,17 +512,19 @@ class Context:
         moves to the cache `to` and its totals to acc_to; to None: in place.
         index: int32 [seqs, layers, kv_heads, keep] or None. The sequences
         then hold min(len, keep) positions (lens is the caller's to update)."""
-        _want(cache.device == self.device and (to is None or to.device == self.device), "the cache is on another device")
         if to is None:
             to, acc_to = cache, acc
-        _want(acc_to is None or acc is not None, "acc_to is given without acc")
-        e = EvictArgs(keep, sinks, recent, *cache._acc(acc), *to._acc(acc_to, "acc_to"), stream=_stream(stream))
+        if cache.device != self.device or to.device != self.device:
+            raise MingError("the cache is on another device")
+        i = 0
         if index is not None:
-            _tensor(index, "index", "torch.int32", 4, self.device)
-            _want(tuple(index.shape) == (cache.args.seqs, cache.args.layers, cache.args.kv_heads, keep) and
-                  index.is_contiguous(), "index: contiguous [seqs, layers, kv_heads, keep] is wanted")
-            e.index = index.data_ptr()
-        _check(lib().ming_cuda_kv_evict(self._h, cache.ref, to.ref, ctypes.addressof(e)))
+            _tensor(index, "index", _types()[2], 4, self.device)
+            if index.shape != cache.shape + (keep,) or not index.is_contiguous():
+                raise MingError("index: contiguous [seqs, layers, kv_heads, keep] is wanted")
+            i = index.data_ptr()
+        _EVICT.pack_into(self._args, 0, keep, sinks, recent, *cache._acc(acc), *to._acc(acc_to, "acc_to"), i,
+                         0 if stream is None else stream or 1)
+        _check(lib().ming_cuda_kv_evict(self._h, cache.ref, to.ref, self._args_at))
 
     def unpack_linear(self, weight_name, out_dim, in_dim):
         out = np.empty((out_dim, in_dim), dtype=np.float32)
