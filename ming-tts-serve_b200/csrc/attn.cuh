@@ -67,6 +67,13 @@ cudaError_t launch_attn_weights(const AttnOp& a, cudaStream_t s);
 cudaError_t launch_attn_decode(const AttnOp& a, cudaStream_t s);
 cudaError_t launch_kv_evict(const EvictOp& a, cudaStream_t s);
 
+// Two f32 rounded to bf16 (to nearest, ties to even), lo in the low half.
+MING_DEV uint32_t at_bf16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
 MING_DEV void at_flag(int* err, int code) {
     if (err) atomicCAS(err, 0, code);
 }

@@ -187,9 +187,9 @@ __global__ void __launch_bounds__(DE_THREADS, 2) attn_decode_kernel(const AttnOp
 #pragma unroll
         for (int d = 0; d < 4; d++) e[d] = exp2f(c[d] - m);
         l += (e[0] + e[1]) + (e[2] + e[3]);
-        const uint32_t h0 = pack_bf16x2(e[0], e[1]), h1 = pack_bf16x2(e[2], e[3]);
+        const uint32_t h0 = at_bf16x2(e[0], e[1]), h1 = at_bf16x2(e[2], e[3]);
         const float2 f0 = unpack_bf16x2(h0), f1 = unpack_bf16x2(h1);
-        const uint32_t pa[4] = {h0, pack_bf16x2(e[0] - f0.x, e[1] - f0.y), h1, pack_bf16x2(e[2] - f1.x, e[3] - f1.y)};
+        const uint32_t pa[4] = {h0, at_bf16x2(e[0] - f0.x, e[1] - f0.y), h1, at_bf16x2(e[2] - f1.x, e[3] - f1.y)};
         const uint32_t vw[4][4] = {{v[0].x, v[1].x, v[2].x, v[3].x}, {v[0].y, v[1].y, v[2].y, v[3].y},
                                    {v[0].z, v[1].z, v[2].z, v[3].z}, {v[0].w, v[1].w, v[2].w, v[3].w}};
 #pragma unroll
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(DE_THREADS, 2) attn_decode_kernel(const AttnOp
             y += v.y * f;
         }
         const float il = L > 0.f ? 1.f / L : 0.f;
-        reinterpret_cast<uint32_t*>(a.out + b * a.o_rs + (kh * a.group + h) * a.o_hs)[d] = pack_bf16x2(x * il, y * il);
+        reinterpret_cast<uint32_t*>(a.out + b * a.o_rs + (kh * a.group + h) * a.o_hs)[d] = at_bf16x2(x * il, y * il);
     }
     if (MODE != DE_PLAIN) {
         if (tid < AT_MAXG) {
