@@ -1,8 +1,10 @@
 // attn_prefill.cu — attention of a prompt's rows over a paged cache, and the
 // weights that those rows gave to each cached position, on the 5th-generation
 // tensor cores (tcgen05.mma, sums in tensor memory).
+#include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "attn.cuh"
@@ -16,9 +18,8 @@ constexpr int PF_N = 128;        // cached positions of a block: eight pages
 constexpr int PF_PAGES = PF_N / AT_PAGE;
 constexpr int PF_STAGES = 4;
 constexpr int PF_TILE = PF_M * AT_HD * 2;  // 16 KB: a row of 64 bf16 is one 128-byte swizzled line
-constexpr int PF_THREADS = 384;            // two softmax warpgroups, then one MMA warp and three loading warps
-constexpr int PF_LOADERS = 96;
-constexpr int PF_SMEM = 1024 + 2 * PF_TILE + PF_STAGES * 2 * PF_TILE + 256;
+constexpr int PF_THREADS = 352;            // two softmax warpgroups, then a warp each for products, copies and edges
+constexpr int PF_SMEM = 1024 + 4 * PF_TILE + PF_STAGES * 2 * PF_TILE + 256;
 constexpr long long PF_TIMEOUT = 4000000000LL;  // cycles (~2 s) before a wait gives up; the ones here end in microseconds
 // tensor memory columns
 constexpr int PF_S = 0;    // logits of the two tiles, f32 [128 rows][128]
@@ -99,12 +100,16 @@ MING_DEV void pf_ld32(uint32_t* v, uint32_t addr) {
         : PF_R8(v, 0), PF_R8(v, 8), PF_R8(v, 16), PF_R8(v, 24)
         : "r"(addr));
 }
-MING_DEV void pf_st32(uint32_t addr, const uint32_t* v) {
+MING_DEV void pf_ld16(uint32_t* v, uint32_t addr) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(
-            addr),
-        PF_W8(v, 0), PF_W8(v, 8), PF_W8(v, 16), PF_W8(v, 24)
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+        : PF_R8(v, 0), PF_R8(v, 8)
+        : "r"(addr));
+}
+MING_DEV void pf_st16(uint32_t addr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(addr),
+        PF_W8(v, 0), PF_W8(v, 8)
         : "memory");
 }
 // Waits for the loads into v; the empty statements keep its uses behind the wait.
@@ -189,83 +194,88 @@ struct BlockSpan {
     }
 };
 
-// The loading warps copy one block's keys and values into swizzled tiles, a
-// warp a page at a time, 16 bytes a lane; rows that no row of the CTA sees
-// become zeros (a weight of zero times a stale NaN would be NaN).
-MING_DEV void pf_load_block(const KvPages& kv, const int* bt, const RowsSee& see, int kh, int block, uint8_t* tiles, int lw,
-                            int lane, bool values, int* err) {
-    const int v = block * PF_PAGES + (lane & 7);
-    const int mine = v < see.np ? see.page(v) : -1;
-    const int64_t base = mine >= 0 ? (int64_t)at_page(kv, bt, mine, err) * kv.ps + kh * kv.hs : 0;
-    const int row = lane >> 3, chunk = lane & 7;
-    const int64_t off = row * kv.ss + chunk * 8, step = 4 * kv.ss;
-    const uint32_t at = pf_su32(tiles) + row * 128;
-    const uint32_t c0 = (uint32_t)(chunk ^ row) << 4, c1 = (uint32_t)(chunk ^ (row + 4)) << 4;
-    for (int u = lw; u < (values ? 2 : 1) * PF_PAGES; u += PF_LOADERS / 32) {
-        const int pi = u & (PF_PAGES - 1);
-        const int page = __shfl_sync(0xffffffffu, mine, pi);
-        const uint16_t* s = (u < PF_PAGES ? kv.k : kv.v) + __shfl_sync(0xffffffffu, base, pi) + off;
-        const uint32_t d = at + (u < PF_PAGES ? 0 : PF_TILE) + pi * (AT_PAGE * 128);
-        const int j = page * AT_PAGE + row;
-        const bool whole = page >= 0 && see.all(page);
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const bool live = whole || (page >= 0 && see.any(j + 4 * k));
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(d + k * 512 + (k & 1 ? c1 : c0)), "l"(s + k * step),
-                         "r"(live ? 16 : 0)
-                         : "memory");
-        }
-    }
+MING_DEV void pf_expect(uint64_t* b, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(pf_su32(b)), "r"(bytes) : "memory");
+}
+// A page of one kv head: 16 rows of 128 bytes, swizzled. Page `pages` lies outside the map and gives zeros.
+MING_DEV void pf_copy_page(void* dst, const CUtensorMap* m, int kh, int page, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %3, %4}], [%5];\n" ::"r"(
+            pf_su32(dst)),
+        "l"(reinterpret_cast<uint64_t>(m)), "r"(0), "r"(kh), "r"(page), "r"(pf_su32(bar))
+        : "memory");
+}
+// A tile of q: every head of the group at 128 / group positions from `row` on.
+MING_DEV void pf_copy_q(void* dst, const CUtensorMap* m, int head, int row, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(
+            pf_su32(dst)),
+        "l"(reinterpret_cast<uint64_t>(m)), "r"(0), "r"(head), "r"(row), "r"(pf_su32(bar))
+        : "memory");
 }
 
-// One (position, head) row of q into line r of a swizzled tile, zeros if there is none.
-MING_DEV void pf_load_q(const AttnOp& a, uint8_t* tile, int r, int64_t row, int h, bool has) {
-    const uint4* s = reinterpret_cast<const uint4*>(a.q + row * a.q_rs + h * a.q_hs);
-#pragma unroll
-    for (int c = 0; c < 8; c++)
-        *reinterpret_cast<uint4*>(tile + r * 128 + ((c ^ (r & 7)) << 4)) = has ? s[c] : make_uint4(0, 0, 0, 0);
-}
+// The work of a CTA, one (sequence, kv head, up to two tiles of rows) after
+// another; the sequences' last rows, which see the most, come first.
+struct PfItem {
+    int kh, b, x;     // kv head, row of the batch, which rows
+    int r0, r1, len;  // as read: rows of q, positions held
+    MING_DEV PfItem(const AttnOp& a, int w, int nx) {
+        const int per = a.kv_heads * a.seqs, rest = w % per;
+        x = nx - 1 - w / per;
+        b = rest / a.kv_heads;
+        kh = rest % a.kv_heads;
+        at_rows(a, b, r0, r1);
+        len = at_len(a.kv, at_seq(a.kv, b), a.err);
+    }
+};
+struct PfRows {
+    int i0, p0, here;  // first row within the sequence, its position, rows of the item (<= 0: none)
+    MING_DEV PfRows(const PfItem& w, int step) {
+        i0 = w.x * step;
+        p0 = w.len - (w.r1 - w.r0) + i0;
+        here = min(w.r1 - w.r0 - i0, step);
+    }
+    MING_DEV RowsSee see(const AttnOp& a) const { return RowsSee(max(p0, 0), p0 + here - 1, a.window, a.sinks); }
+};
 
 }  // namespace
 
-// A CTA takes two tiles of 128 rows of one (sequence, kv head): a row is a
-// (position, head of the group) pair, so a block of keys and values serves the
-// whole group and the tile's mask is as narrow as its 128 / group positions.
-// Per block of 128 cached positions and tile: logits S = Q K^T into tensor
-// memory (4 tcgen05.mma), a thread per row reads its 128 logits, keeps the
-// running maximum and sum in registers, writes the weights as bf16 pairs back
-// to tensor memory, and O += P V takes them from there (8 tcgen05.mma with V
-// as the transposed operand, its rows as the pages hold them). Nothing of S or
-// P passes through shared memory, and no row needs a shuffle.
+// One CTA per SM takes items of two tiles of 128 rows of one (sequence, kv
+// head): a row is a (position, head of the group) pair, so a block of keys and
+// values serves the whole group and a tile's mask is as narrow as its
+// 128 / group positions. Per block of 128 cached positions and tile: logits
+// S = Q K^T into tensor memory (4 tcgen05.mma), a thread per row reads its 128
+// logits, keeps the running maximum and sum in registers, writes the weights
+// as bf16 pairs back to tensor memory, and O += P V takes them from there (8
+// tcgen05.mma with V as the transposed operand, its rows as the pages hold
+// them). Nothing of S or P passes through shared memory, and no row needs a
+// shuffle.
 //  * Outputs are rescaled only when a row's maximum has risen by more than 2^8
 //    since the last time (sums and outputs carry the same reference, so the
 //    quotient is exact; weights stay below 2^8).
 //  * P is rounded to bf16, half a step of each weight, because the tensor
 //    cores take bf16 next to V; the row's sum is kept from the unrounded ones.
 //  * Softmax of one tile runs while the other's products do; q.k of the next
-//    block is issued as soon as a tile's logits have been read.
-//  * Three warps bring blocks in with 16-byte cp.async (pages may sit at any
-//    stride), four stages of 32 KB ahead.
-__global__ void __launch_bounds__(PF_THREADS, 1) attn_prefill_kernel(const AttnOp a) {
+//    block, the next item's first among them, is issued as soon as a tile's
+//    logits have been read, so items follow one another without a pause.
+//  * Pages come by TMA, one copy each for keys and values, four blocks ahead;
+//    a warp of its own zeroes the values of positions that no row of the item
+//    sees (a weight of zero times a stale NaN would be NaN) before a block is
+//    handed to the products.
+__global__ void __launch_bounds__(PF_THREADS, 1)
+    attn_prefill_kernel(const AttnOp a, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                        const __grid_constant__ CUtensorMap mv, int tiles_of_item, int nx) {
     extern __shared__ __align__(16) uint8_t pf_raw[];
     uint8_t* smem = pf_raw + ((1024u - (pf_su32(pf_raw) & 1023u)) & 1023u);
-    uint8_t* sq = smem;                    // [2] tiles of q
-    uint8_t* skv = smem + 2 * PF_TILE;     // [stage][K|V]
+    uint8_t* sq = smem;                 // [buffer][tile] of q
+    uint8_t* skv = smem + 4 * PF_TILE;  // [stage][K|V]
     uint64_t* bars = reinterpret_cast<uint64_t*>(skv + PF_STAGES * 2 * PF_TILE);
-    uint64_t *full = bars, *empty = bars + PF_STAGES, *s_full = bars + 2 * PF_STAGES, *s_read = s_full + 2,
-             *p_ready = s_full + 4, *o_full = s_full + 6;
-    uint32_t* slot = reinterpret_cast<uint32_t*>(s_full + 8);
+    uint64_t *landed = bars, *full = bars + PF_STAGES, *empty = bars + 2 * PF_STAGES, *q_full = bars + 3 * PF_STAGES,
+             *q_empty = q_full + 2, *s_full = q_full + 4, *s_read = q_full + 6, *p_ready = q_full + 8, *o_full = q_full + 10;
+    uint32_t* slot = reinterpret_cast<uint32_t*>(q_full + 12);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int kh = blockIdx.y, b = blockIdx.z, G = a.group, per = PF_M / G;  // positions of a tile
-    int r0, r1;
-    at_rows(a, b, r0, r1);
-    const int rows = r1 - r0, x = gridDim.x - 1 - blockIdx.x, i0 = x * 2 * per;  // the longest rows first
-    if (i0 >= rows) return;
-    const int seq = at_seq(a.kv, b), len = at_len(a.kv, seq, a.err), p0 = len - rows + i0;
-    const int* bt = a.kv.bt + (size_t)seq * a.kv.bt_ld;
-    const int here = min(rows - i0, 2 * per), tiles = here > per ? 2 : 1;
-    const RowsSee see(max(p0, 0), p0 + here - 1, a.window, a.sinks);
-    const int nb = see.blocks();
+    const int G = a.group, per = PF_M / G, step = tiles_of_item * per;  // positions of a tile, of an item
+    const int total = nx * a.kv_heads * a.seqs;
 
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(pf_su32(slot)), "r"(PF_COLS)
@@ -274,10 +284,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1) attn_prefill_kernel(const AttnO
     }
     if (tid == 0) {
         for (int i = 0; i < PF_STAGES; i++) {
-            pf_bar_init(&full[i], PF_LOADERS);
+            pf_bar_init(&landed[i], 1);
+            pf_bar_init(&full[i], 1);
             pf_bar_init(&empty[i], 1);
         }
         for (int t = 0; t < 2; t++) {
+            pf_bar_init(&q_full[t], 1);
+            pf_bar_init(&q_empty[t], 1);
             pf_bar_init(&s_full[t], 1);
             pf_bar_init(&s_read[t], 4);
             pf_bar_init(&p_ready[t], 4);
@@ -285,168 +298,255 @@ __global__ void __launch_bounds__(PF_THREADS, 1) attn_prefill_kernel(const AttnO
         }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
-    const int t = warp >> 2;                       // softmax warps: the tile
-    const int r = tid & 127, i = i0 + t * per + r / G, h = kh * G + r % G;
-    const bool has = t < 2 && r < per * G && i < rows;
-    if (t < 2) {
-        pf_load_q(a, sq + t * PF_TILE, r, r0 + i, h, has);
-        pf_async_fence();
-    }
     pf_before();
     __syncthreads();
     pf_after();
     const uint32_t tmem = *slot;
     bool ok = true;
     if (warp == 8) {
-        if (lane == 0 && nb > 0) {
-            auto kv_at = [&](int j) { return pf_su32(skv) + (uint32_t)(j % PF_STAGES) * 2 * PF_TILE; };
-            ok = pf_wait(&full[0], 0);
-            for (int u = 0; ok && u < tiles; u++) {
-                pf_product(tmem + PF_S + u * PF_N, pf_su32(sq) + u * PF_TILE, kv_at(0));
-                pf_commit(&s_full[u]);
-            }
-            for (int j = 0; ok && j < nb; j++) {
-                for (int u = 0; ok && u < tiles; u++) {
-                    if (j + 1 < nb) {
-                        if (u == 0) ok = pf_wait(&full[(j + 1) % PF_STAGES], ((j + 1) / PF_STAGES) & 1);
-                        ok = ok && pf_wait(&s_read[u], j & 1);
-                        if (!ok) break;
-                        pf_after();
-                        pf_product(tmem + PF_S + u * PF_N, pf_su32(sq) + u * PF_TILE, kv_at(j + 1));
-                        pf_commit(&s_full[u]);
-                    }
-                    if (!(ok = pf_wait(&p_ready[u], j & 1))) break;
-                    pf_after();
-#pragma unroll
-                    for (int ks = 0; ks < PF_N / 16; ks++)
-                        pf_mma_ts(tmem + PF_O + u * AT_HD, tmem + PF_P + u * (PF_N / 2) + ks * 8,
-                                  pf_desc(kv_at(j) + PF_TILE + ks * 2048), PF_IDESC_PV, j > 0 || ks > 0);
-                    pf_commit(&o_full[u]);
+        if (lane == 0) {
+            // a cursor over the blocks of all items
+            struct Cursor {
+                int w, nb, tiles, j, q, n;  // item, its blocks and tiles, block of it, items before it, blocks before it
+            } c{(int)blockIdx.x - (int)gridDim.x, 0, 0, -1, -1, -1}, d;
+            auto next = [&](Cursor& k) {
+                k.n++;
+                if (++k.j < k.nb) return true;
+                k.j = 0;
+                k.q++;
+                while ((k.w += gridDim.x) < total) {
+                    const PfItem it(a, k.w, nx);
+                    const PfRows rows(it, step);
+                    if (rows.here <= 0) continue;
+                    k.nb = rows.see(a).blocks();
+                    k.tiles = rows.here > per ? 2 : 1;
+                    if (k.nb > 0) return true;
                 }
-                if (ok) pf_commit(&empty[j % PF_STAGES]);
+                return false;
+            };
+            int reads[2] = {0, 0}, weights[2] = {0, 0};  // q.k products issued, weights' products issued
+            auto kv_at = [&](const Cursor& k) { return pf_su32(skv) + (uint32_t)(k.n % PF_STAGES) * 2 * PF_TILE; };
+            auto logits = [&](const Cursor& k, int u) {
+                if (u == 0 && k.j == 0 && !pf_wait(&q_full[k.q & 1], (k.q >> 1) & 1)) return false;
+                if (u == 0 && !pf_wait(&full[k.n % PF_STAGES], (k.n / PF_STAGES) & 1)) return false;
+                if (reads[u] && !pf_wait(&s_read[u], (reads[u] - 1) & 1)) return false;
+                reads[u]++;
+                pf_after();
+                pf_product(tmem + PF_S + u * PF_N, pf_su32(sq) + (2 * (k.q & 1) + u) * PF_TILE, kv_at(k));
+                pf_commit(&s_full[u]);
+                if (u == k.tiles - 1 && k.j == k.nb - 1) pf_commit(&q_empty[k.q & 1]);
+                return true;
+            };
+            bool more = next(c);
+            for (int u = 0; more && ok && u < c.tiles; u++) ok = logits(c, u);
+            while (more && ok) {
+                d = c;
+                more = next(d);
+                for (int u = 0; ok && u < 2; u++) {
+                    if (more && u < d.tiles) ok = logits(d, u);
+                    if (ok && u < c.tiles) {
+                        if (!(ok = pf_wait(&p_ready[u], weights[u] & 1))) break;
+                        weights[u]++;
+                        pf_after();
+#pragma unroll
+                        for (int ks = 0; ks < PF_N / 16; ks++)
+                            pf_mma_ts(tmem + PF_O + u * AT_HD, tmem + PF_P + u * (PF_N / 2) + ks * 8,
+                                      pf_desc(kv_at(c) + PF_TILE + ks * 2048), PF_IDESC_PV, c.j > 0 || ks > 0);
+                        pf_commit(&o_full[u]);
+                    }
+                }
+                if (ok) pf_commit(&empty[c.n % PF_STAGES]);
+                c = d;
             }
         }
         __syncwarp();
-    } else if (warp > 8) {
-        const int lw = warp - 9;
-        for (int j = 0; ok && j <= nb; j++) {
-            if (j < nb) {
-                if (j >= PF_STAGES) ok = pf_wait_warp(&empty[j % PF_STAGES], ((j / PF_STAGES) - 1) & 1);
-                if (ok) {
-                    uint8_t* st = skv + (j % PF_STAGES) * 2 * PF_TILE;
-                    pf_load_block(a.kv, bt, see, kh, j, st, lw, lane, true, a.err);
-                }
+    } else if (warp == 9) {
+        int n = 0, q = 0;
+        for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
+            const PfItem it(a, w, nx);
+            const PfRows rows(it, step);
+            if (rows.here <= 0) continue;
+            const RowsSee see = rows.see(a);
+            const int nb = see.blocks(), tiles = rows.here > per ? 2 : 1;
+            if (nb == 0) continue;
+            const int* bt = a.kv.bt + (size_t)at_seq(a.kv, it.b) * a.kv.bt_ld;
+            // lanes 0-7 and 8-15 (keys, values) take a page each
+            auto look_up = [&](int j) {
+                const int v = j * PF_PAGES + (lane & 7);
+                return v < see.np ? at_page(a.kv, bt, see.page(v), a.err) : a.kv.pages;
+            };
+            int page = look_up(0);
+            if (q >= 2) ok = pf_wait_warp(&q_empty[q & 1], ((q >> 1) - 1) & 1);
+            if (!ok) break;
+            if (lane == 0) {
+                pf_expect(&q_full[q & 1], (uint32_t)(tiles * per * G * 128));
+                for (int u = 0; u < tiles; u++)
+                    pf_copy_q(sq + (2 * (q & 1) + u) * PF_TILE, &mq, it.kh * G, it.r0 + rows.i0 + u * per, &q_full[q & 1]);
             }
-            asm volatile("cp.async.commit_group;\n" ::: "memory");
-            if (j > 0) {
-                // the block before this one is in: hand it over
-                asm volatile("cp.async.wait_group 1;\n" ::: "memory");
-                pf_async_fence();
-                pf_arrive(&full[(j - 1) % PF_STAGES]);
+            q++;
+            for (int j = 0; j < nb; j++, n++) {
+                const int st = n % PF_STAGES, now = page;
+                if (j + 1 < nb) page = look_up(j + 1);
+                if (n >= PF_STAGES && !(ok = pf_wait_warp(&empty[st], ((n / PF_STAGES) - 1) & 1))) break;
+                if (lane == 0) pf_expect(&landed[st], 2 * PF_TILE);
+                __syncwarp();
+                if (lane < 2 * PF_PAGES)
+                    pf_copy_page(skv + st * 2 * PF_TILE + (lane >> 3) * PF_TILE + (lane & 7) * (AT_PAGE * 128), lane < 8 ? &mk : &mv,
+                                 it.kh, now, &landed[st]);
             }
         }
-        asm volatile("cp.async.wait_group 0;\n" ::: "memory");
-    } else if (t < tiles) {
+    } else if (warp == 10) {
+        int n = 0;
+        for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
+            const PfItem it(a, w, nx);
+            const PfRows rows(it, step);
+            if (rows.here <= 0) continue;
+            const RowsSee see = rows.see(a);
+            const int nb = see.blocks();
+            for (int j = 0; j < nb; j++, n++) {
+                const int st = n % PF_STAGES;
+                if (!(ok = pf_wait_warp(&landed[st], (n / PF_STAGES) & 1))) break;
+                uint8_t* tile = skv + st * 2 * PF_TILE + PF_TILE;
+                for (int i = 0; i < PF_PAGES && j * PF_PAGES + i < see.np; i++) {
+                    const int page = see.page(j * PF_PAGES + i);
+                    if (see.all(page)) continue;
+                    for (int k = lane >> 3; k < AT_PAGE; k += 4)
+                        if (!see.any(page * AT_PAGE + k))
+                            *reinterpret_cast<uint4*>(tile + (i * AT_PAGE + k) * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                }
+                pf_async_fence();
+                __syncwarp();
+                if (lane == 0) pf_arrive(&full[st]);
+            }
+        }
+    } else {
+        const int t = warp >> 2, r = tid & 127, rp = r / G, rh = r % G;  // the tile, its row's position and head
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + PF_S + t * PF_N, tp = tmem + lanes + PF_P + t * (PF_N / 2),
                        to = tmem + lanes + PF_O + t * AT_HD;
-        const int p = has ? p0 + t * per + r / G : -1;
-        const int pa = p0 + t * per, pb = p0 + min(here, (t + 1) * per) - 1;
-        float m = -INFINITY, l = 0.f;  // reference maximum (of q.k) and sum of the weights against it
-        for (int j = 0; j < nb; j++) {
-            if (!(ok = pf_wait_warp(&s_full[t], j & 1))) break;
-            pf_after();
-            uint32_t s[PF_N];
-#pragma unroll
-            for (int c = 0; c < PF_N; c += 32) pf_ld32(s + c, ts + c);
-            pf_wait_ld(s);
-            pf_before();
-            __syncwarp();
-            if (lane == 0) pf_arrive(&s_read[t]);
-            const BlockSpan span(see, j);
-            if (!span.whole(pa, pb, a.window, a.sinks)) {
-#pragma unroll
-                for (int c = 0; c < PF_N; c += 32) {
+        int n = 0;  // blocks of this tile so far
+        for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
+            const PfItem it(a, w, nx);
+            const PfRows rows(it, step);
+            if (rows.here <= t * per) continue;
+            const RowsSee see = rows.see(a);
+            const int nb = see.blocks(), h = it.kh * G + rh, i = rows.i0 + t * per + rp;
+            const bool has = r < per * G && t * per + rp < rows.here;
+            const int pa = rows.p0 + t * per, pb = rows.p0 + min(rows.here, (t + 1) * per) - 1, p = has ? pa + rp : -1;
+            float m = -INFINITY, l = 0.f;  // reference maximum (of q.k) and sum of the weights against it
+            for (int j = 0; j < nb; j++, n++) {
+                if (!(ok = pf_wait_warp(&s_full[t], n & 1))) break;
+                pf_after();
+                const BlockSpan span(see, j);
+                const bool whole = span.whole(pa, pb, a.window, a.sinks);
+                // the row's logits, 32 columns at a time, twice: the maximum
+                // first, then the weights against it (reading tensor memory
+                // again costs less than 128 registers)
+                uint32_t s[2][32];
+                auto masked = [&](uint32_t (&v)[32], int c) {
+                    if (whole) return;
                     const uint32_t bits = span.sees(c, p, a.window, a.sinks);
 #pragma unroll
                     for (int e = 0; e < 32; e++)
-                        if (!((bits >> e) & 1u)) s[c + e] = 0xff800000u;  // -infinity
+                        if (!((bits >> e) & 1u)) v[e] = 0xff800000u;  // -infinity
+                };
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                pf_ld32(s[0], ts);
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    pf_wait_ld(s[c & 1]);
+                    pf_ld32(s[(c + 1) & 1], ts + ((c + 1) & 3) * 32);
+                    masked(s[c & 1], c * 32);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8)
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            mx[k] = fmaxf(mx[k], fmaxf(__uint_as_float(s[c & 1][e + 2 * k]), __uint_as_float(s[c & 1][e + 2 * k + 1])));
                 }
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                float f = 1.f;
+                const bool rise = top > m && (top - m) * a.scale_log2 > 8.f;  // also from -infinity
+                if (rise) {
+                    f = m == -INFINITY ? 0.f : pf_ex2((m - top) * a.scale_log2);
+                    m = top;
+                    l *= f;
+                }
+                if (j > 0) {
+                    if (!(ok = pf_wait_warp(&o_full[t], (n - 1) & 1))) break;  // the last block's product has read P and written O
+                    pf_after();
+                    if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+                        for (int c = 0; c < AT_HD; c += 16) {
+                            uint32_t o[16];
+                            pf_ld16(o, to + c);
+                            pf_wait_ld(o);
+#pragma unroll
+                            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            pf_st16(to + c, o);
+                        }
+                    }
+                }
+                const float ref = m == -INFINITY ? 0.f : -m * a.scale_log2;
+                const uint64_t sc2 = pf_pair(a.scale_log2, a.scale_log2), ref2 = pf_pair(ref, ref);
+                uint64_t sum[2] = {0ull, 0ull};
+                pf_wait_ld(s[0]);
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    uint32_t (&v)[32] = s[c & 1];
+                    if (c > 0) pf_wait_ld(v);
+                    if (c < 3) pf_ld32(s[(c + 1) & 1], ts + (c + 1) * 32);
+                    else {
+                        pf_before();
+                        __syncwarp();
+                        if (lane == 0) pf_arrive(&s_read[t]);
+                    }
+                    masked(v, c * 32);
+                    uint32_t wt[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        float e0, e1;
+                        pf_unpair(pf_fma2(pf_pair(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), sc2, ref2), e0, e1);
+                        e0 = pf_ex2(e0);
+                        e1 = pf_ex2(e1);
+                        sum[(e >> 1) & 1] = pf_add2(sum[(e >> 1) & 1], pf_pair(e0, e1));
+                        wt[e / 2] = at_bf16x2(e0, e1);
+                    }
+                    pf_st16(tp + c * 16, wt);
+                }
+                float u0, u1;
+                pf_unpair(pf_add2(sum[0], sum[1]), u0, u1);
+                l += u0 + u1;
+                pf_wait_st();
+                pf_before();
+                __syncwarp();
+                if (lane == 0) pf_arrive(&p_ready[t]);
             }
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (ok && nb > 0) ok = pf_wait_warp(&o_full[t], (n - 1) & 1);
+            pf_after();
+            const float il = ok && l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
-            for (int c = 0; c < PF_N; c += 8)
+            for (int c = 0; c < AT_HD; c += 32) {
+                uint32_t o[32];
+                pf_ld32(o, to + c);
+                pf_wait_ld(o);
+                if (has) {
+                    uint4* d = reinterpret_cast<uint4*>(a.out + (int64_t)(it.r0 + i) * a.o_rs + h * a.o_hs + c);
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    mx[e] = fmaxf(mx[e], fmaxf(__uint_as_float(s[c + 2 * e]), __uint_as_float(s[c + 2 * e + 1])));
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-            float f = 1.f;
-            const bool rise = top > m && (top - m) * a.scale_log2 > 8.f;  // also from -infinity
-            if (rise) {
-                f = m == -INFINITY ? 0.f : pf_ex2((m - top) * a.scale_log2);
-                m = top;
-                l *= f;
-            }
-            const float ref = m == -INFINITY ? 0.f : -m * a.scale_log2;
-            const uint64_t sc2 = pf_pair(a.scale_log2, a.scale_log2), ref2 = pf_pair(ref, ref);
-            uint64_t sum[2] = {0ull, 0ull};
-            uint32_t w[PF_N / 2];
+                    for (int e = 0; e < 32; e += 8) {
+                        uint32_t y[4];
 #pragma unroll
-            for (int c = 0; c < PF_N; c += 2) {
-                float e0, e1;
-                pf_unpair(pf_fma2(pf_pair(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc2, ref2), e0, e1);
-                e0 = pf_ex2(e0);
-                e1 = pf_ex2(e1);
-                sum[(c >> 1) & 1] = pf_add2(sum[(c >> 1) & 1], pf_pair(e0, e1));
-                w[c / 2] = at_bf16x2(e0, e1);
-            }
-            float u0, u1;
-            pf_unpair(pf_add2(sum[0], sum[1]), u0, u1);
-            l += u0 + u1;
-            if (j > 0) {
-                if (!(ok = pf_wait_warp(&o_full[t], (j - 1) & 1))) break;  // the last block's product has read P and written O
-                pf_after();
-                if (__any_sync(0xffffffffu, rise)) {
-#pragma unroll
-                    for (int c = 0; c < AT_HD; c += 32) {
-                        uint32_t o[32];
-                        pf_ld32(o, to + c);
-                        pf_wait_ld(o);
-#pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        pf_st32(to + c, o);
+                        for (int k = 0; k < 4; k++)
+                            // nothing seen: zeros, whatever the tensor memory held
+                            y[k] = l > 0.f || l != l ? at_bf16x2(__uint_as_float(o[e + 2 * k]) * il, __uint_as_float(o[e + 2 * k + 1]) * il)
+                                                     : 0u;
+                        d[e / 8] = make_uint4(y[0], y[1], y[2], y[3]);
                     }
                 }
             }
-            pf_st32(tp, w);
-            pf_st32(tp + 32, w + 32);
-            pf_wait_st();
-            pf_before();
-            __syncwarp();
-            if (lane == 0) pf_arrive(&p_ready[t]);
+            if (has && a.lse)
+                a.lse[(size_t)(it.r0 + i) * a.heads + h] = l == 0.f ? -INFINITY : (m * a.scale_log2 + log2f(l)) / AT_LOG2E;
+            pf_before();  // the next item's products may write O once its weights are announced
         }
-        if (ok && nb > 0) ok = pf_wait_warp(&o_full[t], (nb - 1) & 1);
-        pf_after();
-        const float il = ok && l > 0.f ? 1.f / l : 0.f;
-#pragma unroll
-        for (int c = 0; c < AT_HD; c += 32) {
-            uint32_t o[32];
-            pf_ld32(o, to + c);
-            pf_wait_ld(o);
-            if (has) {
-                uint4* d = reinterpret_cast<uint4*>(a.out + (int64_t)(r0 + i) * a.o_rs + h * a.o_hs + c);
-#pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                    uint32_t y[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        // nothing seen: zeros, whatever the tensor memory held
-                        y[k] = l > 0.f || l != l ? at_bf16x2(__uint_as_float(o[e + 2 * k]) * il, __uint_as_float(o[e + 2 * k + 1]) * il) : 0u;
-                    d[e / 8] = make_uint4(y[0], y[1], y[2], y[3]);
-                }
-            }
-        }
-        if (has && a.lse) a.lse[(size_t)(r0 + i) * a.heads + h] = l == 0.f ? -INFINITY : (m * a.scale_log2 + log2f(l)) / AT_LOG2E;
     }
     if (!ok) at_flag(a.err, AT_ERR_WAIT);
     pf_before();
@@ -482,6 +582,46 @@ __global__ void __launch_bounds__(128) attn_weights_kernel(const AttnOp a) {
     *t = (j >= first ? 0.f : *t) + w;
 }
 
+namespace {
+constexpr int SMS = 148;
+
+bool encode(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims, const int64_t* strides, const cuuint32_t* box) {
+    using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+                       q == cudaDriverEntryPointSuccess
+                   ? reinterpret_cast<Encode>(f)
+                   : nullptr;
+    }();
+    if (!fn) return false;
+    cuuint64_t st[4];
+    // a dimension that is never stepped over may come with stride 0, which a map does not take
+    for (int i = 0; i + 1 < rank; i++) st[i] = dims[i + 1] == 1 ? 16 : (cuuint64_t)strides[i] * 2;
+    const cuuint32_t one[4] = {1, 1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, st, box, one,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// K or V of one layer as [page][kv head][slot][dim], a box a page of one head
+bool page_map(CUtensorMap* m, const KvPages& kv, const uint16_t* base, int kv_heads) {
+    const cuuint64_t dims[4] = {AT_HD, AT_PAGE, (cuuint64_t)kv_heads, (cuuint64_t)kv.pages};
+    const int64_t st[3] = {kv.ss, kv.hs, kv.ps};
+    const cuuint32_t box[4] = {AT_HD, AT_PAGE, 1, 1};
+    return encode(m, base, 4, dims, st, box);
+}
+// q as [row][head][dim], a box the heads of a group at `per` rows
+bool q_map(CUtensorMap* m, const AttnOp& a, int per) {
+    const cuuint64_t dims[3] = {AT_HD, (cuuint64_t)a.heads, (cuuint64_t)a.rows};
+    const int64_t st[2] = {a.q_hs, a.q_rs};
+    const cuuint32_t box[3] = {AT_HD, (cuuint32_t)a.group, (cuuint32_t)per};
+    return encode(m, a.q, 3, dims, st, box);
+}
+}  // namespace
+
 cudaError_t launch_attn_prefill(const AttnOp& a, cudaStream_t s) {
     static std::atomic<bool> ready[64] = {};  // per device: the kernel's attribute is set
     int dev = 0;
@@ -492,8 +632,18 @@ cudaError_t launch_attn_prefill(const AttnOp& a, cudaStream_t s) {
             return e;
         if (dev < 64) ready[dev].store(true, std::memory_order_release);
     }
-    const int per = 2 * (PF_M / a.group);
-    attn_prefill_kernel<<<dim3((a.max_rows + per - 1) / per, a.kv_heads, a.seqs), PF_THREADS, PF_SMEM, s>>>(a);
+    const int per = PF_M / a.group;
+    CUtensorMap mq, mk, mv;
+    if (!q_map(&mq, a, per) || !page_map(&mk, a.kv, a.kv.k, a.kv_heads) || !page_map(&mv, a.kv, a.kv.v, a.kv_heads))
+        return cudaErrorInvalidValue;
+    // items of one tile while every one of them finds an SM: the latency of a
+    // block is then one tile's
+    const long long heads = (long long)a.kv_heads * a.seqs, one = (long long)((a.max_rows + per - 1) / per) * heads;
+    const int tiles = one <= SMS ? 1 : 2;
+    const int nx = (a.max_rows + tiles * per - 1) / (tiles * per);
+    if (nx * heads > 0x7fffffff) return cudaErrorInvalidValue;
+    const int grid = (int)std::min<long long>(SMS, nx * heads);
+    attn_prefill_kernel<<<grid, PF_THREADS, PF_SMEM, s>>>(a, mq, mk, mv, tiles, nx);
     return cudaGetLastError();
 }
 
