@@ -22,9 +22,9 @@ constexpr int PF_THREADS = 352;            // two softmax warpgroups, then a war
 constexpr int PF_SMEM = 1024 + 4 * PF_TILE + PF_STAGES * 2 * PF_TILE + 256;
 constexpr long long PF_TIMEOUT = 4000000000LL;  // cycles (~2 s) before a wait gives up; the ones here end in microseconds
 // tensor memory columns
-constexpr int PF_S = 0;    // logits of the two tiles, f32 [128 rows][128]
-constexpr int PF_P = 256;  // weights of the two tiles, bf16 pairs [128 rows][64]
-constexpr int PF_O = 384;  // outputs of the two tiles, f32 [128 rows][64]
+constexpr int PF_BUFS = 3;  // logits of three (block, tile) steps, f32 [128 rows][128]; a step's weights replace its
+                            // logits, bf16 pairs [128 rows][64]
+constexpr int PF_O = 384;   // outputs of the two tiles, f32 [128 rows][64]
 constexpr int PF_COLS = 512;
 
 MING_DEV uint32_t pf_su32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -55,6 +55,11 @@ MING_DEV bool pf_wait_warp(uint64_t* b, uint32_t parity) { return __all_sync(0xf
 MING_DEV void pf_commit(uint64_t* b) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(pf_su32(b)) : "memory");
 }
+MING_DEV bool pf_elect() {
+    uint32_t one;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}\n" : "=r"(one));
+    return one != 0;
+}
 MING_DEV void pf_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 MING_DEV void pf_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
 MING_DEV void pf_async_fence() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
@@ -65,6 +70,9 @@ MING_DEV void pf_async_fence() { asm volatile("fence.proxy.async.shared::cta;\n"
 MING_DEV uint64_t pf_desc(uint32_t saddr) {
     return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
            ((uint64_t)2 << 61);
+}
+MING_DEV uint64_t pf_desc_lo(uint32_t addr16) {  // of an address in units of 16 bytes
+    return (uint64_t)(addr16 & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 // Instruction descriptors (kind::f16): f32 sums, bf16 operands, M 128; B
 // K-major of N 128 for q.k, B transposed of N 64 for the weights' product.
@@ -105,6 +113,14 @@ MING_DEV void pf_ld16(uint32_t* v, uint32_t addr) {
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
         : PF_R8(v, 0), PF_R8(v, 8)
         : "r"(addr));
+}
+MING_DEV void pf_st32(uint32_t addr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(
+            addr),
+        PF_W8(v, 0), PF_W8(v, 8), PF_W8(v, 16), PF_W8(v, 24)
+        : "memory");
 }
 MING_DEV void pf_st16(uint32_t addr, const uint32_t* v) {
     asm volatile(
@@ -264,17 +280,18 @@ struct PfRows {
 //    handed to the products.
 __global__ void __launch_bounds__(PF_THREADS, 1)
     attn_prefill_kernel(const AttnOp a, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
-                        const __grid_constant__ CUtensorMap mv, int tiles_of_item, int nx) {
+                        const __grid_constant__ CUtensorMap mv, int tiles, int nx) {
     extern __shared__ __align__(16) uint8_t pf_raw[];
     uint8_t* smem = pf_raw + ((1024u - (pf_su32(pf_raw) & 1023u)) & 1023u);
     uint8_t* sq = smem;                 // [buffer][tile] of q
     uint8_t* skv = smem + 4 * PF_TILE;  // [stage][K|V]
     uint64_t* bars = reinterpret_cast<uint64_t*>(skv + PF_STAGES * 2 * PF_TILE);
     uint64_t *landed = bars, *full = bars + PF_STAGES, *empty = bars + 2 * PF_STAGES, *q_full = bars + 3 * PF_STAGES,
-             *q_empty = q_full + 2, *s_full = q_full + 4, *s_read = q_full + 6, *p_ready = q_full + 8, *o_full = q_full + 10;
-    uint32_t* slot = reinterpret_cast<uint32_t*>(q_full + 12);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int G = a.group, per = PF_M / G, step = tiles_of_item * per;  // positions of a tile, of an item
+             *q_empty = q_full + 2, *s_full = q_full + 4, *p_ready = s_full + PF_BUFS, *o_full = p_ready + PF_BUFS;
+    uint32_t* slot = reinterpret_cast<uint32_t*>(o_full + 2);
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be the same in every lane
+    const int G = a.group, per = PF_M / G, step = tiles * per;  // positions of a tile, of an item
     const int total = nx * a.kv_heads * a.seqs;
 
     if (warp == 8) {
@@ -291,10 +308,11 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         for (int t = 0; t < 2; t++) {
             pf_bar_init(&q_full[t], 1);
             pf_bar_init(&q_empty[t], 1);
-            pf_bar_init(&s_full[t], 1);
-            pf_bar_init(&s_read[t], 4);
-            pf_bar_init(&p_ready[t], 4);
             pf_bar_init(&o_full[t], 1);
+        }
+        for (int i = 0; i < PF_BUFS; i++) {
+            pf_bar_init(&s_full[i], 1);
+            pf_bar_init(&p_ready[i], 4);
         }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -304,62 +322,88 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     const uint32_t tmem = *slot;
     bool ok = true;
     if (warp == 8) {
-        if (lane == 0) {
-            // a cursor over the blocks of all items
-            struct Cursor {
-                int w, nb, tiles, j, q, n;  // item, its blocks and tiles, block of it, items before it, blocks before it
-            } c{(int)blockIdx.x - (int)gridDim.x, 0, 0, -1, -1, -1}, d;
-            auto next = [&](Cursor& k) {
-                k.n++;
-                if (++k.j < k.nb) return true;
-                k.j = 0;
-                k.q++;
-                while ((k.w += gridDim.x) < total) {
-                    const PfItem it(a, k.w, nx);
-                    const PfRows rows(it, step);
-                    if (rows.here <= 0) continue;
-                    k.nb = rows.see(a).blocks();
-                    k.tiles = rows.here > per ? 2 : 1;
-                    if (k.nb > 0) return true;
-                }
-                return false;
-            };
-            int reads[2] = {0, 0}, weights[2] = {0, 0};  // q.k products issued, weights' products issued
-            auto kv_at = [&](const Cursor& k) { return pf_su32(skv) + (uint32_t)(k.n % PF_STAGES) * 2 * PF_TILE; };
-            auto logits = [&](const Cursor& k, int u) {
-                if (u == 0 && k.j == 0 && !pf_wait(&q_full[k.q & 1], (k.q >> 1) & 1)) return false;
-                if (u == 0 && !pf_wait(&full[k.n % PF_STAGES], (k.n / PF_STAGES) & 1)) return false;
-                if (reads[u] && !pf_wait(&s_read[u], (reads[u] - 1) & 1)) return false;
-                reads[u]++;
-                pf_after();
-                pf_product(tmem + PF_S + u * PF_N, pf_su32(sq) + (2 * (k.q & 1) + u) * PF_TILE, kv_at(k));
-                pf_commit(&s_full[u]);
-                if (u == k.tiles - 1 && k.j == k.nb - 1) pf_commit(&q_empty[k.q & 1]);
-                return true;
-            };
-            bool more = next(c);
-            for (int u = 0; more && ok && u < c.tiles; u++) ok = logits(c, u);
-            while (more && ok) {
-                d = c;
-                more = next(d);
-                for (int u = 0; ok && u < 2; u++) {
-                    if (more && u < d.tiles) ok = logits(d, u);
-                    if (ok && u < c.tiles) {
-                        if (!(ok = pf_wait(&p_ready[u], weights[u] & 1))) break;
-                        weights[u]++;
-                        pf_after();
-#pragma unroll
-                        for (int ks = 0; ks < PF_N / 16; ks++)
-                            pf_mma_ts(tmem + PF_O + u * AT_HD, tmem + PF_P + u * (PF_N / 2) + ks * 8,
-                                      pf_desc(kv_at(c) + PF_TILE + ks * 2048), PF_IDESC_PV, c.j > 0 || ks > 0);
-                        pf_commit(&o_full[u]);
-                    }
-                }
-                if (ok) pf_commit(&empty[c.n % PF_STAGES]);
-                c = d;
+        // The whole warp runs this role and one elected lane issues: the
+        // descriptors then stay in uniform registers (a lone lane's products
+        // went out at 71 and 57 cycles each, these at 65 and 36).
+        const bool lead = pf_elect();
+        const uint32_t lo_q = pf_su32(sq) >> 4, lo_kv = pf_su32(skv) >> 4;
+        // the next step, a (block, tile), to compute logits for
+        int w = (int)blockIdx.x - (int)gridDim.x, nb = 0, j = 0, u = 0, stage = 0, stage_phase = 0, q = -1;
+        auto next_item = [&]() {
+            j = 0;
+            q++;
+            while ((w += gridDim.x) < total) {
+                const PfItem it(a, w, nx);
+                const PfRows rows(it, step);
+                if (rows.here <= 0) continue;
+                nb = rows.see(a).blocks();
+                if (nb > 0) return true;
             }
+            return false;
+        };
+        bool more = next_item();
+        // What the weights' product of each buffer needs, noted with its
+        // logits: stage, tile, whether it adds to O, whether it is the block's last.
+        int note[PF_BUFS];
+        uint32_t phase = 0;
+        // Products run in the order of their issue: a step's logits follow the
+        // product that read the weights in the same buffer.
+        auto logits = [&](int buf) {
+            if (u == 0) {
+                if (j == 0 && !pf_wait_warp(&q_full[q & 1], (q >> 1) & 1)) return false;
+                if (!pf_wait_warp(&full[stage], stage_phase)) return false;
+            }
+            pf_after();
+            const bool last = u == tiles - 1;
+            if (lead) {
+                const uint64_t dq = pf_desc_lo(lo_q + (uint32_t)(2 * (q & 1) + u) * (PF_TILE >> 4)),
+                               dk = pf_desc_lo(lo_kv + (uint32_t)stage * (2 * PF_TILE >> 4));
+#pragma unroll
+                for (int ks = 0; ks < 4; ks++) pf_mma_ss(tmem + buf * PF_N, dq + 2 * ks, dk + 2 * ks, PF_IDESC_QK, ks > 0);
+                pf_commit(&s_full[buf]);
+                if (last && j == nb - 1) pf_commit(&q_empty[q & 1]);
+            }
+            __syncwarp();
+            note[buf] = stage | u << 4 | (j > 0 ? 32 : 0) | (last ? 64 : 0);
+            if (last) {
+                u = 0;
+                if (++stage == PF_STAGES) {
+                    stage = 0;
+                    stage_phase ^= 1;
+                }
+                if (++j == nb) more = next_item();
+            } else {
+                u++;
+            }
+            return true;
+        };
+#pragma unroll
+        for (int i = 0; i < PF_BUFS; i++) {
+            note[i] = -1;
+            if (more && ok) ok = logits(i);
         }
-        __syncwarp();
+        while (ok && note[0] >= 0) {
+#pragma unroll
+            for (int buf = 0; buf < PF_BUFS; buf++) {
+                const int k = note[buf];
+                if (!ok || k < 0) continue;
+                if (!(ok = pf_wait_warp(&p_ready[buf], phase))) continue;
+                pf_after();
+                if (lead) {
+                    const uint64_t dv = pf_desc_lo(lo_kv + (uint32_t)(k & 15) * (2 * PF_TILE >> 4) + (PF_TILE >> 4));
+                    const uint32_t o = tmem + PF_O + ((k >> 4) & 1) * AT_HD;
+#pragma unroll
+                    for (int ks = 0; ks < PF_N / 16; ks++)
+                        pf_mma_ts(o, tmem + buf * PF_N + ks * 8, dv + ks * (2048 >> 4), PF_IDESC_PV, (k & 32) || ks > 0);
+                    pf_commit(&o_full[(k >> 4) & 1]);
+                    if (k & 64) pf_commit(&empty[k & 15]);
+                }
+                __syncwarp();
+                note[buf] = -1;
+                if (more) ok = logits(buf);
+            }
+            phase ^= 1;
+        }
     } else if (warp == 9) {
         int n = 0, q = 0;
         for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
@@ -367,7 +411,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
             const PfRows rows(it, step);
             if (rows.here <= 0) continue;
             const RowsSee see = rows.see(a);
-            const int nb = see.blocks(), tiles = rows.here > per ? 2 : 1;
+            const int nb = see.blocks();
             if (nb == 0) continue;
             const int* bt = a.kv.bt + (size_t)at_seq(a.kv, it.b) * a.kv.bt_ld;
             // lanes 0-7 and 8-15 (keys, values) take a page each
@@ -419,30 +463,41 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                 if (lane == 0) pf_arrive(&full[st]);
             }
         }
-    } else {
+    } else if (warp < 4 * tiles) {
         const int t = warp >> 2, r = tid & 127, rp = r / G, rh = r % G;  // the tile, its row's position and head
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + lanes + PF_S + t * PF_N, tp = tmem + lanes + PF_P + t * (PF_N / 2),
-                       to = tmem + lanes + PF_O + t * AT_HD;
-        int n = 0;  // blocks of this tile so far
+        const uint32_t to = tmem + lanes + PF_O + t * AT_HD;
+        int n = 0, g0 = 0;  // blocks of this tile so far, steps of the items so far
         for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
             const PfItem it(a, w, nx);
             const PfRows rows(it, step);
-            if (rows.here <= t * per) continue;
+            if (rows.here <= 0) continue;
             const RowsSee see = rows.see(a);
-            const int nb = see.blocks(), h = it.kh * G + rh, i = rows.i0 + t * per + rp;
+            const int nb = see.blocks();
+            int g = g0 + t;  // this tile's step
+            g0 += nb * tiles;
+            const int h = it.kh * G + rh, i = rows.i0 + t * per + rp;
             const bool has = r < per * G && t * per + rp < rows.here;
             const int pa = rows.p0 + t * per, pb = rows.p0 + min(rows.here, (t + 1) * per) - 1, p = has ? pa + rp : -1;
-            float m = -INFINITY, l = 0.f;  // reference maximum (of q.k) and sum of the weights against it
-            for (int j = 0; j < nb; j++, n++) {
-                if (!(ok = pf_wait_warp(&s_full[t], n & 1))) break;
+            const float most = 8.f / a.scale_log2;  // a rise of q.k that weights may carry (infinite at scale 0)
+            float m = -INFINITY, l = 0.f;           // reference maximum (of q.k) and sum of the weights against it
+            for (int j = 0; j < nb; j++, n++, g += tiles) {
+                const int buf = g % PF_BUFS;
+                const uint32_t ts = tmem + lanes + buf * PF_N;
+                if (!(ok = pf_wait_warp(&s_full[buf], (g / PF_BUFS) & 1))) break;
+                // The last item of a sequence may leave its second tile empty:
+                // its steps are taken, so that every warpgroup sees every
+                // phase of its barriers, but nothing is computed.
+                if (pb < pa) {
+                    if (j > 0 && !(ok = pf_wait_warp(&o_full[t], (n - 1) & 1))) break;
+                    __syncwarp();
+                    if (lane == 0) pf_arrive(&p_ready[buf]);
+                    continue;
+                }
                 pf_after();
                 const BlockSpan span(see, j);
                 const bool whole = span.whole(pa, pb, a.window, a.sinks);
-                // the row's logits, 32 columns at a time, twice: the maximum
-                // first, then the weights against it (reading tensor memory
-                // again costs less than 128 registers)
-                uint32_t s[2][32];
+                uint32_t s[2][32], wt[PF_N / 2];  // 32 logits in use, 32 on their way; the weights
                 auto masked = [&](uint32_t (&v)[32], int c) {
                     if (whole) return;
                     const uint32_t bits = span.sees(c, p, a.window, a.sinks);
@@ -451,30 +506,65 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                         if (!((bits >> e) & 1u)) v[e] = 0xff800000u;  // -infinity
                 };
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                pf_ld32(s[0], ts);
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    pf_wait_ld(s[c & 1]);
-                    pf_ld32(s[(c + 1) & 1], ts + ((c + 1) & 3) * 32);
-                    masked(s[c & 1], c * 32);
+                auto highest = [&](const uint32_t (&v)[32]) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 8)
 #pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            mx[k] = fmaxf(mx[k], fmaxf(__uint_as_float(s[c & 1][e + 2 * k]), __uint_as_float(s[c & 1][e + 2 * k + 1])));
-                }
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                float f = 1.f;
-                const bool rise = top > m && (top - m) * a.scale_log2 > 8.f;  // also from -infinity
-                if (rise) {
-                    f = m == -INFINITY ? 0.f : pf_ex2((m - top) * a.scale_log2);
-                    m = top;
-                    l *= f;
-                }
-                if (j > 0) {
-                    if (!(ok = pf_wait_warp(&o_full[t], (n - 1) & 1))) break;  // the last block's product has read P and written O
-                    pf_after();
+                        for (int k = 0; k < 4; k++) mx[k] = fmaxf(mx[k], fmaxf(__uint_as_float(v[e + 2 * k]), __uint_as_float(v[e + 2 * k + 1])));
+                };
+                // Weights against the reference as it stands, and the block's
+                // maximum on the way: one pass, unless a row's maximum has risen
+                // too far (its first block, seldom after), then a second one.
+                uint64_t sum[2];
+                auto weigh = [&](bool look) {
+                    const float ref = m == -INFINITY ? 0.f : -m * a.scale_log2;
+                    const uint64_t sc2 = pf_pair(a.scale_log2, a.scale_log2), ref2 = pf_pair(ref, ref);
+                    sum[0] = sum[1] = 0ull;
+                    pf_ld32(s[0], ts);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        uint32_t (&v)[32] = s[c & 1];
+                        pf_wait_ld(v);
+                        if (c < 3) pf_ld32(s[(c + 1) & 1], ts + (c + 1) * 32);
+                        masked(v, c * 32);
+                        if (look) highest(v);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            float e0, e1;
+                            pf_unpair(pf_fma2(pf_pair(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), sc2, ref2), e0, e1);
+                            e0 = pf_ex2(e0);
+                            e1 = pf_ex2(e1);
+                            sum[(e >> 1) & 1] = pf_add2(sum[(e >> 1) & 1], pf_pair(e0, e1));
+                            wt[c * 16 + e / 2] = at_bf16x2(e0, e1);
+                        }
+                    }
+                };
+                if (j == 0) {
+                    pf_ld32(s[0], ts);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        pf_wait_ld(s[c & 1]);
+                        if (c < 3) pf_ld32(s[(c + 1) & 1], ts + (c + 1) * 32);
+                        masked(s[c & 1], c * 32);
+                        highest(s[c & 1]);
+                    }
+                    m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    weigh(false);
+                } else {
+                    weigh(true);
+                    // the last block's product has written O (waited for every
+                    // time: a parity names a phase only if none is left out)
+                    if (!(ok = pf_wait_warp(&o_full[t], (n - 1) & 1))) break;
+                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    const bool rise = top > m && (m == -INFINITY || top - m > most);
                     if (__any_sync(0xffffffffu, rise)) {
+                        float f = 1.f;
+                        if (rise) {
+                            f = m == -INFINITY ? 0.f : pf_ex2((m - top) * a.scale_log2);
+                            m = top;
+                            l *= f;
+                        }
+                        pf_after();
 #pragma unroll
                         for (int c = 0; c < AT_HD; c += 16) {
                             uint32_t o[16];
@@ -484,42 +574,18 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                             for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
                             pf_st16(to + c, o);
                         }
+                        weigh(false);
                     }
                 }
-                const float ref = m == -INFINITY ? 0.f : -m * a.scale_log2;
-                const uint64_t sc2 = pf_pair(a.scale_log2, a.scale_log2), ref2 = pf_pair(ref, ref);
-                uint64_t sum[2] = {0ull, 0ull};
-                pf_wait_ld(s[0]);
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    uint32_t (&v)[32] = s[c & 1];
-                    if (c > 0) pf_wait_ld(v);
-                    if (c < 3) pf_ld32(s[(c + 1) & 1], ts + (c + 1) * 32);
-                    else {
-                        pf_before();
-                        __syncwarp();
-                        if (lane == 0) pf_arrive(&s_read[t]);
-                    }
-                    masked(v, c * 32);
-                    uint32_t wt[16];
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        float e0, e1;
-                        pf_unpair(pf_fma2(pf_pair(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), sc2, ref2), e0, e1);
-                        e0 = pf_ex2(e0);
-                        e1 = pf_ex2(e1);
-                        sum[(e >> 1) & 1] = pf_add2(sum[(e >> 1) & 1], pf_pair(e0, e1));
-                        wt[e / 2] = at_bf16x2(e0, e1);
-                    }
-                    pf_st16(tp + c * 16, wt);
-                }
+                pf_st32(ts, wt);
+                pf_st32(ts + 32, wt + 32);
                 float u0, u1;
                 pf_unpair(pf_add2(sum[0], sum[1]), u0, u1);
                 l += u0 + u1;
                 pf_wait_st();
                 pf_before();
                 __syncwarp();
-                if (lane == 0) pf_arrive(&p_ready[t]);
+                if (lane == 0) pf_arrive(&p_ready[buf]);
             }
             if (ok && nb > 0) ok = pf_wait_warp(&o_full[t], (n - 1) & 1);
             pf_after();

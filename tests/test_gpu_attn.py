@@ -230,6 +230,14 @@ def test_prefill_long(ctx):
     check_prefill(ctx, Case([9000, 4100], [40, 18], 14, 2, 5000, 4, seed=12))
 
 
+@pytest.mark.parametrize("window,sinks", [(0, 0), (70, 4)])
+@pytest.mark.parametrize("lens", [[509, 287, 497, 507, 477, 233, 3, 358, 1], [130] * 40, [5] * 200, [700] * 7 + [19] * 30])
+def test_prefill_many_sequences(ctx, lens, window, sinks):
+    """More work than SMs: a CTA takes several items, of both full and odd tiles."""
+    check_prefill(ctx, Case(lens, lens, 14, 2, window, sinks, seed=len(lens)))
+    check_prefill(ctx, Case(lens, [(n + 1) // 2 for n in lens], 16, 2, window, sinks, seed=len(lens)))
+
+
 def test_prefill_sharp(ctx):
     """Logits of hundreds: a row's weight sits on one or two positions and its maximum keeps rising."""
     check_prefill(ctx, Case([600], [600], 14, 2, 0, 0, sharp=60.0, seed=13))
