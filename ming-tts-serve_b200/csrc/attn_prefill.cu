@@ -37,9 +37,9 @@ MING_DEV void pf_arrive(uint64_t* b) {
 MING_DEV bool pf_try(uint64_t* b, uint32_t parity) {
     uint32_t ok;
     asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
         : "=r"(ok)
-        : "r"(pf_su32(b)), "r"(parity)
+        : "r"(pf_su32(b)), "r"(parity), "r"(1000000)  // sleeps up to a millisecond instead of spinning beside warps at work
         : "memory");
     return ok != 0;
 }
@@ -342,67 +342,76 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
             return false;
         };
         bool more = next_item();
-        // What the weights' product of each buffer needs, noted with its
-        // logits: stage, tile, whether it adds to O, whether it is the block's last.
-        int note[PF_BUFS];
+        // The step's operands are in
+        auto ready = [&]() {
+            if (u) return true;
+            if (j == 0 && !pf_wait_warp(&q_full[q & 1], (q >> 1) & 1)) return false;
+            return pf_wait_warp(&full[stage], stage_phase);
+        };
+        auto logits = [&](int buf) {  // by the elected lane
+            const uint32_t dq = lo_q + (uint32_t)(2 * (q & 1) + u) * (PF_TILE >> 4), dk = lo_kv + (uint32_t)stage * (2 * PF_TILE >> 4);
+#pragma unroll
+            for (int ks = 0; ks < 4; ks++) pf_mma_ss(tmem + buf * PF_N, pf_desc_lo(dq + 2 * ks), pf_desc_lo(dk + 2 * ks), PF_IDESC_QK, ks > 0);
+            pf_commit(&s_full[buf]);
+            if (u == tiles - 1 && j == nb - 1) pf_commit(&q_empty[q & 1]);
+        };
+        // What a step's weights' product needs, noted with its logits: stage,
+        // tile, whether it adds to O, whether it is the block's last; then the
+        // cursor moves on.
+        auto note = [&]() {
+            const bool last = u == tiles - 1;
+            const int k = stage | u << 4 | (j > 0 ? 32 : 0) | (last ? 64 : 0);
+            u = last ? 0 : 1;
+            if (last) {
+                stage = (stage + 1) % PF_STAGES;
+                stage_phase ^= stage == 0;
+                if (++j == nb) more = next_item();
+            }
+            return k;
+        };
+        // The steps between their two products, PF_BUFS at most, oldest first.
+        // A compact loop: this warp runs its few instructions once a step,
+        // between the softmax warps' long ones, and each miss in the
+        // instruction cache is on the way of both.
+        int note0 = -1, note1 = -1, note2 = -1;
+#pragma unroll 1
+        for (int buf = 0; buf < PF_BUFS; buf++) {
+            if (!more) break;
+            if (!(ok = ready())) break;
+            pf_after();
+            if (lead) logits(buf);
+            __syncwarp();
+            (buf == 0 ? note0 : buf == 1 ? note1 : note2) = note();
+        }
+        int buf = 0;
         uint32_t phase = 0;
         // Products run in the order of their issue: a step's logits follow the
         // product that read the weights in the same buffer.
-        auto logits = [&](int buf) {
-            if (u == 0) {
-                if (j == 0 && !pf_wait_warp(&q_full[q & 1], (q >> 1) & 1)) return false;
-                if (!pf_wait_warp(&full[stage], stage_phase)) return false;
-            }
+#pragma unroll 1
+        while (ok && note0 >= 0) {
+            const bool follows = more;
+            if (follows && !(ok = ready())) break;
+            if (!(ok = pf_wait_warp(&p_ready[buf], phase))) break;
             pf_after();
-            const bool last = u == tiles - 1;
             if (lead) {
-                const uint64_t dq = pf_desc_lo(lo_q + (uint32_t)(2 * (q & 1) + u) * (PF_TILE >> 4)),
-                               dk = pf_desc_lo(lo_kv + (uint32_t)stage * (2 * PF_TILE >> 4));
+                const uint32_t dv = lo_kv + (uint32_t)(note0 & 15) * (2 * PF_TILE >> 4) + (PF_TILE >> 4), v = (note0 >> 4) & 1;
+                // a block's weights: 32 positions in 16 columns, then 16 free ones
 #pragma unroll
-                for (int ks = 0; ks < 4; ks++) pf_mma_ss(tmem + buf * PF_N, dq + 2 * ks, dk + 2 * ks, PF_IDESC_QK, ks > 0);
-                pf_commit(&s_full[buf]);
-                if (last && j == nb - 1) pf_commit(&q_empty[q & 1]);
+                for (int ks = 0; ks < PF_N / 16; ks++)
+                    pf_mma_ts(tmem + PF_O + v * AT_HD, tmem + buf * PF_N + (ks >> 1) * 32 + (ks & 1) * 8, pf_desc_lo(dv + ks * (2048 >> 4)),
+                              PF_IDESC_PV, (note0 & 32) || ks > 0);
+                pf_commit(&o_full[v]);
+                if (note0 & 64) pf_commit(&empty[note0 & 15]);
+                if (follows) logits(buf);
             }
             __syncwarp();
-            note[buf] = stage | u << 4 | (j > 0 ? 32 : 0) | (last ? 64 : 0);
-            if (last) {
-                u = 0;
-                if (++stage == PF_STAGES) {
-                    stage = 0;
-                    stage_phase ^= 1;
-                }
-                if (++j == nb) more = next_item();
-            } else {
-                u++;
+            note0 = note1;
+            note1 = note2;
+            note2 = follows ? note() : -1;
+            if (++buf == PF_BUFS) {
+                buf = 0;
+                phase ^= 1;
             }
-            return true;
-        };
-#pragma unroll
-        for (int i = 0; i < PF_BUFS; i++) {
-            note[i] = -1;
-            if (more && ok) ok = logits(i);
-        }
-        while (ok && note[0] >= 0) {
-#pragma unroll
-            for (int buf = 0; buf < PF_BUFS; buf++) {
-                const int k = note[buf];
-                if (!ok || k < 0) continue;
-                if (!(ok = pf_wait_warp(&p_ready[buf], phase))) continue;
-                pf_after();
-                if (lead) {
-                    const uint64_t dv = pf_desc_lo(lo_kv + (uint32_t)(k & 15) * (2 * PF_TILE >> 4) + (PF_TILE >> 4));
-                    const uint32_t o = tmem + PF_O + ((k >> 4) & 1) * AT_HD;
-#pragma unroll
-                    for (int ks = 0; ks < PF_N / 16; ks++)
-                        pf_mma_ts(o, tmem + buf * PF_N + ks * 8, dv + ks * (2048 >> 4), PF_IDESC_PV, (k & 32) || ks > 0);
-                    pf_commit(&o_full[(k >> 4) & 1]);
-                    if (k & 64) pf_commit(&empty[k & 15]);
-                }
-                __syncwarp();
-                note[buf] = -1;
-                if (more) ok = logits(buf);
-            }
-            phase ^= 1;
         }
     } else if (warp == 9) {
         int n = 0, q = 0;
@@ -497,75 +506,40 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                 pf_after();
                 const BlockSpan span(see, j);
                 const bool whole = span.whole(pa, pb, a.window, a.sinks);
-                uint32_t s[2][32], wt[PF_N / 2];  // 32 logits in use, 32 on their way; the weights
-                auto masked = [&](uint32_t (&v)[32], int c) {
-                    if (whole) return;
-                    const uint32_t bits = span.sees(c, p, a.window, a.sinks);
+                uint32_t s[PF_N];
 #pragma unroll
-                    for (int e = 0; e < 32; e++)
-                        if (!((bits >> e) & 1u)) v[e] = 0xff800000u;  // -infinity
-                };
+                for (int c = 0; c < PF_N; c += 32) pf_ld32(s + c, ts + c);
+                pf_wait_ld(s);
+                if (!whole) {
+#pragma unroll
+                    for (int c = 0; c < PF_N; c += 32) {
+                        const uint32_t bits = span.sees(c, p, a.window, a.sinks);
+#pragma unroll
+                        for (int e = 0; e < 32; e++)
+                            if (!((bits >> e) & 1u)) s[c + e] = 0xff800000u;  // -infinity
+                    }
+                }
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                auto highest = [&](const uint32_t (&v)[32]) {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 8)
+                for (int c = 0; c < PF_N; c += 8)
 #pragma unroll
-                        for (int k = 0; k < 4; k++) mx[k] = fmaxf(mx[k], fmaxf(__uint_as_float(v[e + 2 * k]), __uint_as_float(v[e + 2 * k + 1])));
-                };
-                // Weights against the reference as it stands, and the block's
-                // maximum on the way: one pass, unless a row's maximum has risen
-                // too far (its first block, seldom after), then a second one.
-                uint64_t sum[2];
-                auto weigh = [&](bool look) {
-                    const float ref = m == -INFINITY ? 0.f : -m * a.scale_log2;
-                    const uint64_t sc2 = pf_pair(a.scale_log2, a.scale_log2), ref2 = pf_pair(ref, ref);
-                    sum[0] = sum[1] = 0ull;
-                    pf_ld32(s[0], ts);
-#pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        uint32_t (&v)[32] = s[c & 1];
-                        pf_wait_ld(v);
-                        if (c < 3) pf_ld32(s[(c + 1) & 1], ts + (c + 1) * 32);
-                        masked(v, c * 32);
-                        if (look) highest(v);
-#pragma unroll
-                        for (int e = 0; e < 32; e += 2) {
-                            float e0, e1;
-                            pf_unpair(pf_fma2(pf_pair(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), sc2, ref2), e0, e1);
-                            e0 = pf_ex2(e0);
-                            e1 = pf_ex2(e1);
-                            sum[(e >> 1) & 1] = pf_add2(sum[(e >> 1) & 1], pf_pair(e0, e1));
-                            wt[c * 16 + e / 2] = at_bf16x2(e0, e1);
-                        }
+                    for (int e = 0; e < 4; e++)
+                        mx[e] = fmaxf(mx[e], fmaxf(__uint_as_float(s[c + 2 * e]), __uint_as_float(s[c + 2 * e + 1])));
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                const bool rise = top > m && (m == -INFINITY || top - m > most);
+                // the last block's product has written O (waited for every
+                // time: a parity names a phase only if none is left out)
+                if (j > 0 && !(ok = pf_wait_warp(&o_full[t], (n - 1) & 1))) break;
+                if (__any_sync(0xffffffffu, rise)) {
+                    float f = 1.f;
+                    if (rise) {
+                        f = m == -INFINITY ? 0.f : pf_ex2((m - top) * a.scale_log2);
+                        m = top;
+                        l *= f;
                     }
-                };
-                if (j == 0) {
-                    pf_ld32(s[0], ts);
-#pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        pf_wait_ld(s[c & 1]);
-                        if (c < 3) pf_ld32(s[(c + 1) & 1], ts + (c + 1) * 32);
-                        masked(s[c & 1], c * 32);
-                        highest(s[c & 1]);
-                    }
-                    m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                    weigh(false);
-                } else {
-                    weigh(true);
-                    // the last block's product has written O (waited for every
-                    // time: a parity names a phase only if none is left out)
-                    if (!(ok = pf_wait_warp(&o_full[t], (n - 1) & 1))) break;
-                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                    const bool rise = top > m && (m == -INFINITY || top - m > most);
-                    if (__any_sync(0xffffffffu, rise)) {
-                        float f = 1.f;
-                        if (rise) {
-                            f = m == -INFINITY ? 0.f : pf_ex2((m - top) * a.scale_log2);
-                            m = top;
-                            l *= f;
-                        }
+                    if (j > 0) {
                         pf_after();
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < AT_HD; c += 16) {
                             uint32_t o[16];
                             pf_ld16(o, to + c);
@@ -574,11 +548,25 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                             for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
                             pf_st16(to + c, o);
                         }
-                        weigh(false);
                     }
                 }
-                pf_st32(ts, wt);
-                pf_st32(ts + 32, wt + 32);
+                const float ref = m == -INFINITY ? 0.f : -m * a.scale_log2;
+                const uint64_t sc2 = pf_pair(a.scale_log2, a.scale_log2), ref2 = pf_pair(ref, ref);
+                uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll
+                for (int c = 0; c < PF_N; c += 32) {
+                    uint32_t wt[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        float e0, e1;
+                        pf_unpair(pf_fma2(pf_pair(__uint_as_float(s[c + e]), __uint_as_float(s[c + e + 1])), sc2, ref2), e0, e1);
+                        e0 = pf_ex2(e0);
+                        e1 = pf_ex2(e1);
+                        sum[(e >> 1) & 1] = pf_add2(sum[(e >> 1) & 1], pf_pair(e0, e1));
+                        wt[e / 2] = at_bf16x2(e0, e1);
+                    }
+                    pf_st16(ts + c, wt);
+                }
                 float u0, u1;
                 pf_unpair(pf_add2(sum[0], sum[1]), u0, u1);
                 l += u0 + u1;
