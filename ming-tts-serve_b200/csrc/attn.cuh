@@ -78,15 +78,15 @@ MING_DEV void at_flag(int* err, int code) {
     if (err) atomicCAS(err, 0, code);
 }
 MING_DEV int at_seq(const KvPages& kv, int b) { return kv.seq_ids ? kv.seq_ids[b] : b; }
-// The sequence's positions, clamped into [0, max_len].
-MING_DEV int at_len(const KvPages& kv, int seq, int* err) {
-    const int n = kv.lens[seq] + kv.len_add;
+// A sequence's positions, clamped into [0, max_len].
+MING_DEV int at_len(const KvPages& kv, int n, int* err) {
     if (n < 0 || n > kv.max_len) {
         at_flag(err, AT_ERR_LEN);
         return n < 0 ? 0 : kv.max_len;
     }
     return n;
 }
+MING_DEV int at_len_of(const KvPages& kv, int seq, int* err) { return at_len(kv, kv.lens[seq] + kv.len_add, err); }
 // The page that holds page-index i of a sequence's table row, 0 if the entry
 // lies outside the pool.
 MING_DEV int at_page(const KvPages& kv, const int* row, int i, int* err) {
@@ -95,10 +95,8 @@ MING_DEV int at_page(const KvPages& kv, const int* row, int i, int* err) {
     at_flag(err, AT_ERR_PAGE);
     return 0;
 }
-// A sequence's rows [r0, r1) of q, clamped into [0, rows] and to max_rows.
-MING_DEV void at_rows(const AttnOp& a, int b, int& r0, int& r1) {
-    r0 = a.q_start[b];
-    r1 = a.q_start[b + 1];
+// A sequence's rows [r0, r1) of q as q_start gives them, clamped into [0, rows] and to max_rows.
+MING_DEV void at_rows(const AttnOp& a, int& r0, int& r1) {
     if (r0 < 0 || r1 > a.rows || r1 < r0 || r1 - r0 > a.max_rows) {
         at_flag(a.err, AT_ERR_ROWS);
         r0 = min(max(r0, 0), a.rows);

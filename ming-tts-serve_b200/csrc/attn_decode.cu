@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(DE_THREADS, 2) attn_decode_kernel(const AttnOp
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int seq = at_seq(a.kv, b);
     const int* bt = a.kv.bt + (size_t)seq * a.kv.bt_ld;
-    const SeenPages see(at_len(a.kv, seq, a.err), a.window, a.sinks);
+    const SeenPages see(at_len_of(a.kv, seq, a.err), a.window, a.sinks);
     const int v0 = (int)((long long)see.np * rank / ns), v1 = (int)((long long)see.np * (rank + 1) / ns);
 
     // q fragments: row g, dims 8 t + 2 ks.. and 32 + 8 t + 2 ks..

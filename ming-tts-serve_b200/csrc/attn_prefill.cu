@@ -19,7 +19,7 @@ constexpr int PF_PAGES = PF_N / AT_PAGE;
 constexpr int PF_STAGES = 4;
 constexpr int PF_TILE = PF_M * AT_HD * 2;  // 16 KB: a row of 64 bf16 is one 128-byte swizzled line
 constexpr int PF_THREADS = 352;            // two softmax warpgroups, then a warp each for products, copies and edges
-constexpr int PF_SMEM = 1024 + 4 * PF_TILE + PF_STAGES * 2 * PF_TILE + 256;
+constexpr int PF_SMEM = 1024 + 4 * PF_TILE + PF_STAGES * 2 * PF_TILE + 2 * PF_TILE + 256;
 constexpr long long PF_TIMEOUT = 4000000000LL;  // cycles (~2 s) before a wait gives up; the ones here end in microseconds
 // tensor memory columns
 constexpr int PF_BUFS = 3;  // logits of three (block, tile) steps, f32 [128 rows][128]; a step's weights replace its
@@ -235,13 +235,36 @@ MING_DEV void pf_copy_q(void* dst, const CUtensorMap* m, int head, int row, uint
 struct PfItem {
     int kh, b, x;     // kv head, row of the batch, which rows
     int r0, r1, len;  // as read: rows of q, positions held
-    MING_DEV PfItem(const AttnOp& a, int w, int nx) {
+    MING_DEV PfItem() {}
+    // The loads alone: their checks wait until the item's turn.
+    MING_DEV void read(const AttnOp& a, int w, int nx) {
         const int per = a.kv_heads * a.seqs, rest = w % per;
         x = nx - 1 - w / per;
         b = rest / a.kv_heads;
         kh = rest % a.kv_heads;
-        at_rows(a, b, r0, r1);
-        len = at_len(a.kv, at_seq(a.kv, b), a.err);
+        r0 = a.q_start[b];
+        r1 = a.q_start[b + 1];
+        len = a.kv.lens[at_seq(a.kv, b)];
+    }
+    MING_DEV void check(const AttnOp& a) {
+        at_rows(a, r0, r1);
+        len = at_len(a.kv, len + a.kv.len_add, a.err);
+    }
+};
+// A CTA's items in turn, each read while the one before it is worked on.
+struct PfItems {
+    const AttnOp& a;
+    int w, nx, total;
+    PfItem ahead;
+    MING_DEV PfItems(const AttnOp& a_, int nx_, int total_) : a(a_), w(blockIdx.x), nx(nx_), total(total_) {
+        if (w < total) ahead.read(a, w, nx);
+    }
+    MING_DEV bool next(PfItem& it) {
+        if (w >= total) return false;
+        it = ahead;
+        if ((w += gridDim.x) < total) ahead.read(a, w, nx);
+        it.check(a);
+        return true;
     }
 };
 struct PfRows {
@@ -285,12 +308,18 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     uint8_t* smem = pf_raw + ((1024u - (pf_su32(pf_raw) & 1023u)) & 1023u);
     uint8_t* sq = smem;                 // [buffer][tile] of q
     uint8_t* skv = smem + 4 * PF_TILE;  // [stage][K|V]
-    uint64_t* bars = reinterpret_cast<uint64_t*>(skv + PF_STAGES * 2 * PF_TILE);
+    uint8_t* so = skv + PF_STAGES * 2 * PF_TILE;  // [tile] outputs on their way, swizzled
+    uint64_t* bars = reinterpret_cast<uint64_t*>(so + 2 * PF_TILE);
     uint64_t *landed = bars, *full = bars + PF_STAGES, *empty = bars + 2 * PF_STAGES, *q_full = bars + 3 * PF_STAGES,
              *q_empty = q_full + 2, *s_full = q_full + 4, *p_ready = s_full + PF_BUFS, *o_full = p_ready + PF_BUFS;
     uint32_t* slot = reinterpret_cast<uint32_t*>(o_full + 2);
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be the same in every lane
+    if (warp == 9 && lane == 0) {
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(&mq)) : "memory");
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(&mk)) : "memory");
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(&mv)) : "memory");
+    }
     const int G = a.group, per = PF_M / G, step = tiles * per;  // positions of a tile, of an item
     const int total = nx * a.kv_heads * a.seqs;
 
@@ -316,6 +345,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
+    PfItems items(a, nx, total);  // the first one is on its way meanwhile
+    PfItem it;
     pf_before();
     __syncthreads();
     pf_after();
@@ -328,12 +359,11 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         const bool lead = pf_elect();
         const uint32_t lo_q = pf_su32(sq) >> 4, lo_kv = pf_su32(skv) >> 4;
         // the next step, a (block, tile), to compute logits for
-        int w = (int)blockIdx.x - (int)gridDim.x, nb = 0, j = 0, u = 0, stage = 0, stage_phase = 0, q = -1;
+        int nb = 0, j = 0, u = 0, stage = 0, stage_phase = 0, q = -1;
         auto next_item = [&]() {
             j = 0;
             q++;
-            while ((w += gridDim.x) < total) {
-                const PfItem it(a, w, nx);
+            while (items.next(it)) {
                 const PfRows rows(it, step);
                 if (rows.here <= 0) continue;
                 nb = rows.see(a).blocks();
@@ -415,8 +445,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         }
     } else if (warp == 9) {
         int n = 0, q = 0;
-        for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
-            const PfItem it(a, w, nx);
+        while (ok && items.next(it)) {
             const PfRows rows(it, step);
             if (rows.here <= 0) continue;
             const RowsSee see = rows.see(a);
@@ -450,8 +479,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         }
     } else if (warp == 10) {
         int n = 0;
-        for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
-            const PfItem it(a, w, nx);
+        while (ok && items.next(it)) {
             const PfRows rows(it, step);
             if (rows.here <= 0) continue;
             const RowsSee see = rows.see(a);
@@ -477,8 +505,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t to = tmem + lanes + PF_O + t * AT_HD;
         int n = 0, g0 = 0;  // blocks of this tile so far, steps of the items so far
-        for (int w = blockIdx.x; ok && w < total; w += gridDim.x) {
-            const PfItem it(a, w, nx);
+        while (ok && items.next(it)) {
             const PfRows rows(it, step);
             if (rows.here <= 0) continue;
             const RowsSee see = rows.see(a);
@@ -514,6 +541,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
 #pragma unroll
                     for (int c = 0; c < PF_N; c += 32) {
                         const uint32_t bits = span.sees(c, p, a.window, a.sinks);
+                        if (__all_sync(0xffffffffu, bits == 0xffffffffu)) continue;
 #pragma unroll
                         for (int e = 0; e < 32; e++)
                             if (!((bits >> e) & 1u)) s[c + e] = 0xff800000u;  // -infinity
@@ -578,25 +606,37 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
             if (ok && nb > 0) ok = pf_wait_warp(&o_full[t], (n - 1) & 1);
             pf_after();
             const float il = ok && l > 0.f ? 1.f / l : 0.f;
+            // through shared memory, each warp its own 32 rows, so that eight
+            // lanes store a row's 128 bytes together
+            uint8_t* tile = so + t * PF_TILE + (warp & 3) * 32 * 128;
 #pragma unroll
             for (int c = 0; c < AT_HD; c += 32) {
                 uint32_t o[32];
                 pf_ld32(o, to + c);
                 pf_wait_ld(o);
-                if (has) {
-                    uint4* d = reinterpret_cast<uint4*>(a.out + (int64_t)(it.r0 + i) * a.o_rs + h * a.o_hs + c);
 #pragma unroll
-                    for (int e = 0; e < 32; e += 8) {
-                        uint32_t y[4];
+                for (int e = 0; e < 32; e += 8) {
+                    uint32_t y[4];
 #pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            // nothing seen: zeros, whatever the tensor memory held
-                            y[k] = l > 0.f || l != l ? at_bf16x2(__uint_as_float(o[e + 2 * k]) * il, __uint_as_float(o[e + 2 * k + 1]) * il)
-                                                     : 0u;
-                        d[e / 8] = make_uint4(y[0], y[1], y[2], y[3]);
-                    }
+                    for (int k = 0; k < 4; k++)
+                        // nothing seen: zeros, whatever the tensor memory held
+                        y[k] = l > 0.f || l != l ? at_bf16x2(__uint_as_float(o[e + 2 * k]) * il, __uint_as_float(o[e + 2 * k + 1]) * il) : 0u;
+                    *reinterpret_cast<uint4*>(tile + lane * 128 + ((((c + e) / 8) ^ (lane & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
                 }
             }
+            __syncwarp();
+            const int inv = 65536 / G + 1;  // exact below 128 for groups of at most 8
+            const int first = rows.i0 + t * per, rows_of_tile = min(rows.here - t * per, per) * G;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int q = k * 4 + (lane >> 3), rr = (warp & 3) * 32 + q;  // a row of the tile
+                const int rrp = (rr * inv) >> 16, rrh = rr - rrp * G;         // rr / G, rr % G
+                const uint4 y = *reinterpret_cast<const uint4*>(tile + q * 128 + (((lane & 7) ^ (q & 7)) << 4));
+                if (rr < rows_of_tile)
+                    *reinterpret_cast<uint4*>(a.out + (int64_t)(it.r0 + first + rrp) * a.o_rs + (it.kh * G + rrh) * a.o_hs +
+                                              (lane & 7) * 8) = y;
+            }
+            __syncwarp();
             if (has && a.lse)
                 a.lse[(size_t)(it.r0 + i) * a.heads + h] = l == 0.f ? -INFINITY : (m * a.scale_log2 + log2f(l)) / AT_LOG2E;
             pf_before();  // the next item's products may write O once its weights are announced
@@ -612,9 +652,9 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
 // follow one another.
 __global__ void __launch_bounds__(128) attn_weights_kernel(const AttnOp a) {
     const int b = blockIdx.z, kh = blockIdx.y, j = blockIdx.x * 128 + threadIdx.x;
-    int r0, r1;
-    at_rows(a, b, r0, r1);
-    const int seq = at_seq(a.kv, b), n = at_len(a.kv, seq, a.err), first = n - (r1 - r0);
+    int r0 = a.q_start[b], r1 = a.q_start[b + 1];
+    at_rows(a, r0, r1);
+    const int seq = at_seq(a.kv, b), n = at_len_of(a.kv, seq, a.err), first = n - (r1 - r0);
     if (j >= n) return;
     const int* bt = a.kv.bt + (size_t)seq * a.kv.bt_ld;
     const uint16_t* kr =

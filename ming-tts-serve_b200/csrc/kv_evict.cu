@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(const EvictOp a) {
     __shared__ uint32_t s_prefix;
     __shared__ int s_need, warp_kept[8], warp_ties[8], kept_pos[EV_THREADS];
     const int b = blockIdx.z, layer = blockIdx.y, kh = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int seq = at_seq(a.from, b), n = at_len(a.from, seq, a.err), keep = min(a.keep, n);
+    const int seq = at_seq(a.from, b), n = at_len_of(a.from, seq, a.err), keep = min(a.keep, n);
     const int lo = min(a.sinks, n), hi = max(lo, n - a.recent), need = n > a.keep ? a.keep - lo - (n - hi) : hi - lo;
     const float* acc = a.acc ? a.acc + seq * a.a_ss + layer * a.a_ls + kh * a.a_hs : nullptr;
     float* acc_to = a.acc_to ? a.acc_to + seq * a.t_ss + layer * a.t_ls + kh * a.t_hs : nullptr;
