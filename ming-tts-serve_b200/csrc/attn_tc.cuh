@@ -1,0 +1,210 @@
+// attn_tc.cuh — what the tensor-core attention kernels share (attn_prefill.cu,
+// attn_weights.cu): tcgen05 products, tensor memory, mbarriers, page copies and
+// their tensor maps. Descriptor and instruction encodings follow the PTX ISA's
+// tcgen05 matrix and instruction descriptors.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "attn.cuh"
+
+namespace ming {
+
+constexpr int AT_M = 128;        // rows of a tile: (position, head of the group) pairs
+constexpr int AT_N = 128;        // cached positions of a block: eight pages
+constexpr int AT_BLOCK_PAGES = AT_N / AT_PAGE;
+constexpr int AT_TILE = AT_M * AT_HD * 2;  // 16 KB: a row of 64 bf16 is one 128-byte swizzled line
+constexpr long long AT_TIMEOUT = 4000000000LL;  // cycles (~2 s) before a wait gives up; the ones here end in microseconds
+
+MING_DEV uint32_t at_su32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+MING_DEV void at_bar_init(uint64_t* b, int count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(at_su32(b)), "r"(count) : "memory");
+}
+MING_DEV void at_arrive(uint64_t* b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(at_su32(b)) : "memory");
+}
+MING_DEV bool at_try(uint64_t* b, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(at_su32(b)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+MING_DEV bool at_wait(uint64_t* b, uint32_t parity) {
+    if (at_try(b, parity)) return true;
+    const long long t0 = clock64();
+    while (!at_try(b, parity))
+        if (clock64() - t0 > AT_TIMEOUT) return false;
+    return true;
+}
+// The whole warp waits and agrees on the outcome.
+MING_DEV bool at_wait_warp(uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, at_wait(b, parity)); }
+MING_DEV void at_commit(uint64_t* b) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(at_su32(b)) : "memory");
+}
+MING_DEV bool at_elect() {
+    uint32_t one;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}\n" : "=r"(one));
+    return one != 0;
+}
+MING_DEV void at_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
+MING_DEV void at_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
+MING_DEV void at_async_fence() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+
+// Shared-memory matrix descriptor of a tile of 128-byte rows, 128-byte swizzle,
+// groups of eight rows 1024 bytes apart: as [rows][64 K] (K-major) and, with
+// the instruction's transpose bit, as [K rows][64 columns] alike.
+MING_DEV uint64_t at_desc_lo(uint32_t addr16) {  // of an address in units of 16 bytes
+    return (uint64_t)(addr16 & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// Instruction descriptors (kind::f16): f32 sums, bf16 operands, M 128; B
+// K-major of N 128 for q.k, B transposed of N 64 for the weights' product.
+constexpr uint32_t AT_IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(AT_M >> 4) << 24);
+constexpr uint32_t AT_IDESC_QK = AT_IDESC | ((uint32_t)(AT_N >> 3) << 17);
+constexpr uint32_t AT_IDESC_PV = AT_IDESC | ((uint32_t)(AT_HD >> 3) << 17) | (1u << 16);
+
+MING_DEV void at_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
+}
+MING_DEV void at_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
+}
+#define AT_R8(v, i) "=r"((v)[i]), "=r"((v)[i + 1]), "=r"((v)[i + 2]), "=r"((v)[i + 3]), "=r"((v)[i + 4]), "=r"((v)[i + 5]), "=r"((v)[i + 6]), "=r"((v)[i + 7])
+#define AT_W8(v, i) "r"((v)[i]), "r"((v)[i + 1]), "r"((v)[i + 2]), "r"((v)[i + 3]), "r"((v)[i + 4]), "r"((v)[i + 5]), "r"((v)[i + 6]), "r"((v)[i + 7])
+// 32 columns of the warp's 32 lanes
+MING_DEV void at_ld32(uint32_t* v, uint32_t addr) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+        : AT_R8(v, 0), AT_R8(v, 8), AT_R8(v, 16), AT_R8(v, 24)
+        : "r"(addr));
+}
+MING_DEV void at_ld16(uint32_t* v, uint32_t addr) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+        : AT_R8(v, 0), AT_R8(v, 8)
+        : "r"(addr));
+}
+MING_DEV void at_st32(uint32_t addr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(
+            addr),
+        AT_W8(v, 0), AT_W8(v, 8), AT_W8(v, 16), AT_W8(v, 24)
+        : "memory");
+}
+MING_DEV void at_st16(uint32_t addr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(addr),
+        AT_W8(v, 0), AT_W8(v, 8)
+        : "memory");
+}
+// Waits for the loads into v; the empty statements keep its uses behind the wait.
+template <int N>
+MING_DEV void at_wait_ld(uint32_t (&v)[N]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; i++) asm volatile("" : "+r"(v[i]));
+}
+MING_DEV void at_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+
+MING_DEV float at_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+// Two f32 operations in one instruction
+MING_DEV uint64_t at_pair(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+MING_DEV void at_unpair(uint64_t r, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(x), "=f"(y) : "l"(r)); }
+MING_DEV uint64_t at_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+MING_DEV uint64_t at_add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// bits [a, b) of a word
+MING_DEV uint32_t at_bits(int a, int b) {
+    a = max(a, 0);
+    b = min(b, 32);
+    return b <= a ? 0u : (0xffffffffu >> (32 - b)) & (0xffffffffu << a);
+}
+
+MING_DEV void at_expect(uint64_t* b, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(at_su32(b)), "r"(bytes) : "memory");
+}
+// A page of one kv head: 16 rows of 128 bytes, swizzled. Page `pages` lies outside the map and gives zeros.
+MING_DEV void at_copy_page(void* dst, const CUtensorMap* m, int kh, int page, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %3, %4}], [%5];\n" ::"r"(
+            at_su32(dst)),
+        "l"(reinterpret_cast<uint64_t>(m)), "r"(0), "r"(kh), "r"(page), "r"(at_su32(bar))
+        : "memory");
+}
+// A tile of q: every head of the group at 128 / group positions from `row` on.
+MING_DEV void at_copy_q(void* dst, const CUtensorMap* m, int head, int row, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(
+            at_su32(dst)),
+        "l"(reinterpret_cast<uint64_t>(m)), "r"(0), "r"(head), "r"(row), "r"(at_su32(bar))
+        : "memory");
+}
+
+
+// Host: tensor maps
+constexpr int AT_SMS = 148;
+
+inline bool at_encode(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims, const int64_t* strides, const cuuint32_t* box) {
+    using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+                       q == cudaDriverEntryPointSuccess
+                   ? reinterpret_cast<Encode>(f)
+                   : nullptr;
+    }();
+    if (!fn) return false;
+    cuuint64_t st[4];
+    // a dimension that is never stepped over may come with stride 0, which a map does not take
+    for (int i = 0; i + 1 < rank; i++) st[i] = dims[i + 1] == 1 ? 16 : (cuuint64_t)strides[i] * 2;
+    const cuuint32_t one[4] = {1, 1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, st, box, one,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// K or V of one layer as [page][kv head][slot][dim], a box a page of one head
+inline bool at_page_map(CUtensorMap* m, const KvPages& kv, const uint16_t* base, int kv_heads) {
+    const cuuint64_t dims[4] = {AT_HD, AT_PAGE, (cuuint64_t)kv_heads, (cuuint64_t)kv.pages};
+    const int64_t st[3] = {kv.ss, kv.hs, kv.ps};
+    const cuuint32_t box[4] = {AT_HD, AT_PAGE, 1, 1};
+    return at_encode(m, base, 4, dims, st, box);
+}
+// q as [row][head][dim], a box the heads of a group at `per` rows
+inline bool at_q_map(CUtensorMap* m, const AttnOp& a, int per) {
+    const cuuint64_t dims[3] = {AT_HD, (cuuint64_t)a.heads, (cuuint64_t)a.rows};
+    const int64_t st[2] = {a.q_hs, a.q_rs};
+    const cuuint32_t box[3] = {AT_HD, (cuuint32_t)a.group, (cuuint32_t)per};
+    return at_encode(m, a.q, 3, dims, st, box);
+}
+
+}  // namespace ming
