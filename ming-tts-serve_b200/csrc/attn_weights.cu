@@ -18,8 +18,9 @@ constexpr int WT_STAGES = 2;
 constexpr int WT_THREADS = 192;  // four warps of weights, one of products, one of copies
 constexpr int WT_PER_SM = 4;
 constexpr int WT_MAX_SPLIT = 16;  // CTAs of a cluster
+constexpr int WT_OWNERS = 4;      // ranks that add up the sums of a quarter of the positions each
 constexpr int WT_LSE = AT_M * 4;
-constexpr int WT_SMEM = 1024 + AT_TILE + WT_STAGES * AT_TILE + WT_STAGES * WT_LSE + AT_N * 4 + 128;
+constexpr int WT_SMEM = 1024 + AT_TILE + WT_STAGES * AT_TILE + WT_STAGES * WT_LSE + 128 + WT_MAX_SPLIT * AT_N / WT_OWNERS * 4;
 }  // namespace
 
 // acc[j] (+)= sum over rows i and the group's heads of exp(s_ij - lse_i).
@@ -29,34 +30,38 @@ constexpr int WT_SMEM = 1024 + AT_TILE + WT_STAGES * AT_TILE + WT_STAGES * WT_LS
 // threads. lse (times -log2 e) comes along the columns from shared memory,
 // minus infinity where a column is no row.
 // A cluster takes a tile of 128 cached positions of one (sequence, kv head);
-// its CTAs split the tiles of q that see it and rank by rank their sums meet
-// through distributed shared memory: no atomics, one order of sums.
+// its CTAs split the tiles of q that see it, and their sums go through distributed
+// shared memory to the first ranks, which add them up rank by rank while the
+// others leave: no atomics, one order of sums.
 // Bound by the exponentials, 16 a cycle and SM, one per visible pair: four
-// CTAs share an SM (128 tensor memory columns, 51 KB each) and fill each
-// other's waits, so each keeps one buffer of logits and two tiles of q.
+// CTAs share an SM (128 tensor memory columns and 55 KB each) and fill
+// each other's waits, so each keeps one buffer of logits and two tiles of q.
 __global__ void __launch_bounds__(WT_THREADS, WT_PER_SM)
     attn_weights_kernel(const AttnOp a, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, int split) {
     extern __shared__ __align__(16) uint8_t wt_raw[];
     uint8_t* smem = wt_raw + ((1024u - (at_su32(wt_raw) & 1023u)) & 1023u);
     uint8_t *sk = smem, *sq = smem + AT_TILE;
     float* nlse = reinterpret_cast<float*>(sq + WT_STAGES * AT_TILE);  // [stage][column]
-    float* part = nlse + WT_STAGES * AT_M;                             // this CTA's sums
-    uint64_t *k_full = reinterpret_cast<uint64_t*>(part + AT_N), *q_full = k_full + 1, *q_empty = q_full + WT_STAGES,
-             *s_full = q_empty + WT_STAGES, *s_read = s_full + 1;
+    uint64_t *k_full = reinterpret_cast<uint64_t*>(nlse + WT_STAGES * AT_M), *q_full = k_full + 1,
+             *q_empty = q_full + WT_STAGES, *s_full = q_empty + WT_STAGES, *s_read = s_full + 1;
     uint32_t* slot = reinterpret_cast<uint32_t*>(s_read + 1);
+    float* part = reinterpret_cast<float*>(slot + 4);  // an owner's: [rank][AT_N / owners], all ranks' sums of its positions
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-    const int rank = blockIdx.x % split, j0 = blockIdx.x / split * AT_N, kh = blockIdx.y, b = blockIdx.z;
+    const int rank = blockIdx.x % split, tile = blockIdx.x / split, kh = blockIdx.y, b = blockIdx.z;
     const int G = a.group, per = AT_M / G;
     const int seq = at_seq(a.kv, b);
     int r0 = a.q_start[b], r1 = a.q_start[b + 1];
     const int held = a.kv.lens[seq] + a.kv.len_add;
+    if (warp == 5 && lane == 0) {
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(&mq)) : "memory");
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(&mk)) : "memory");
+    }
     at_rows(a, r0, r1);
     const int len = at_len(a.kv, held, a.err), rows = r1 - r0, first = len - rows;
-    // the rows of the sequence that see any position of the tile (the whole cluster agrees)
-    const int j1 = min(j0 + AT_N, len);
-    const int lo = max(0, j0 - first), hi = a.window && j0 >= a.sinks ? (int)min((long long)rows, (long long)j1 - 1 + a.window - first) : rows;
-    if (j0 >= len || lo >= hi) return;
-    // this CTA's share of the tiles of rows [lo, hi)
+    // the rows of the sequence that see any position of the tile, and this CTA's share of them
+    const int j0 = tile * AT_N, lo = max(0, j0 - first), last = min(j0 + AT_N, len) - 1;
+    const int hi = a.window && j0 >= a.sinks ? (int)min((long long)rows, (long long)last + a.window - first) : rows;
+    if (j0 >= len || lo >= hi) return;  // the whole cluster
     const int nt = (hi - lo + per - 1) / per, t0 = (int)((long long)nt * rank / split), steps = (int)((long long)nt * (rank + 1) / split) - t0;
 
     if (warp == 4) {
@@ -78,10 +83,16 @@ __global__ void __launch_bounds__(WT_THREADS, WT_PER_SM)
         const int st = e / ((AT_M - per * G) * 8), k = e % ((AT_M - per * G) * 8);
         *reinterpret_cast<uint4*>(sq + st * AT_TILE + (per * G + k / 8) * 128 + (k % 8) * 16) = make_uint4(0, 0, 0, 0);
     }
+    // the tile's pages, looked up before they are needed
+    int page = a.kv.pages;
+    if (warp == 5 && lane < AT_BLOCK_PAGES && j0 / AT_PAGE + lane < (len + AT_PAGE - 1) / AT_PAGE)
+        page = at_page(a.kv, a.kv.bt + (size_t)seq * a.kv.bt_ld, j0 / AT_PAGE + lane, a.err);
     at_async_fence();
     at_before();
     __syncthreads();
     at_after();
+    // (the others' memory is written to only when this has completed)
+    if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
     const uint32_t tmem = *slot;
     bool ok = true;
     float total = 0.f;
@@ -106,23 +117,18 @@ __global__ void __launch_bounds__(WT_THREADS, WT_PER_SM)
         }
     } else if (warp == 5) {
         if (steps > 0) {
-            const int* bt = a.kv.bt + (size_t)seq * a.kv.bt_ld;
-            const int pages = (len + AT_PAGE - 1) / AT_PAGE;
             if (lane == 0) at_expect(k_full, AT_TILE);
             __syncwarp();
-            if (lane < AT_BLOCK_PAGES) {
-                const int i = j0 / AT_PAGE + lane;
-                at_copy_page(sk + lane * (AT_PAGE * 128), &mk, kh, i < pages ? at_page(a.kv, bt, i, a.err) : a.kv.pages, k_full);
-            }
+            if (lane < AT_BLOCK_PAGES) at_copy_page(sk + lane * (AT_PAGE * 128), &mk, kh, page, k_full);
         }
 #pragma unroll 1
         for (int s = 0; s < steps; s++) {
-            const int st = s % WT_STAGES, i0 = lo + (t0 + s) * per, n = min(per, rows - i0) * G;  // columns that are rows
+            const int st = s % WT_STAGES, i0 = lo + (t0 + s) * per, m = min(per, rows - i0) * G;  // columns that are rows
             float z[AT_M / 32];
 #pragma unroll
             for (int k = 0; k < AT_M / 32; k++) {
                 const int c = k * 32 + lane;
-                z[k] = c < n ? -AT_LOG2E * a.lse[(size_t)(r0 + i0 + c / G) * a.heads + kh * G + c % G] : -INFINITY;
+                z[k] = c < m ? -AT_LOG2E * a.lse[(size_t)(r0 + i0 + c / G) * a.heads + kh * G + c % G] : -INFINITY;
             }
             if (s >= WT_STAGES && !(ok = at_wait_warp(&q_empty[st], ((s / WT_STAGES) - 1) & 1))) break;
             if (lane == 0) {
@@ -136,71 +142,75 @@ __global__ void __launch_bounds__(WT_THREADS, WT_PER_SM)
         }
     } else {
         const uint32_t ts = tmem + ((uint32_t)(warp * 32) << 16);
-        const int j = j0 + tid;
         const uint64_t sc2 = at_pair(a.scale_log2, a.scale_log2);
+        const int j = j0 + tid;
 #pragma unroll 1
-        for (int s = 0; s < steps; s++) {
-            const int st = s % WT_STAGES, i0 = lo + (t0 + s) * per;
-            // the tile's rows that see position j, as columns; everyone's, if no one leaves any out
-            const int c_lo = max(0, j - first - i0) * G;
-            const int c_hi = min(min(per, rows - i0), a.window && j >= a.sinks ? max(0, (int)min((long long)per, (long long)j + a.window - first - i0)) : per) * G;
-            const bool whole = __all_sync(0xffffffffu, c_lo == 0 && c_hi == per * G);
-            if (!(ok = at_wait_warp(s_full, s & 1))) break;
-            at_after();
-            uint64_t sum[2] = {0ull, 0ull};
-            const float* nl = nlse + st * AT_M;
+                    for (int s = 0; s < steps; s++) {
+                        const int st = s % WT_STAGES, i0 = lo + (t0 + s) * per;
+                        // the tile's rows that see position j, as columns; everyone's, if no one leaves any out
+                        const int c_lo = max(0, j - first - i0) * G;
+                        const int seen = a.window && j >= a.sinks ? (int)min((long long)per, (long long)j + a.window - first - i0) : per;
+                        const int c_hi = max(0, min(min(per, rows - i0), seen)) * G;
+                        const bool whole = __all_sync(0xffffffffu, c_lo == 0 && c_hi == per * G);
+                        if (!(ok = at_wait_warp(s_full, s & 1))) break;
+                        at_after();
+                        uint64_t sum[2] = {0ull, 0ull};
+                        const float* nl = nlse + st * AT_M;
 #pragma unroll 1
-            for (int c = 0; c < AT_M; c += 32) {
-                uint32_t v[32];
-                at_ld32(v, ts + c);
-                at_wait_ld(v);
-                if (c == AT_M - 32) {
-                    at_before();
-                    __syncwarp();
-                    if (lane == 0) at_arrive(s_read);
-                }
-                if (!whole) {
-                    const uint32_t bits = at_bits(c_lo - c, c_hi - c);
+                        for (int c = 0; c < AT_M; c += 32) {
+                            uint32_t v[32];
+                            at_ld32(v, ts + c);
+                            at_wait_ld(v);
+                            if (c == AT_M - 32) {
+                                at_before();
+                                __syncwarp();
+                                if (lane == 0) at_arrive(s_read);
+                            }
+                            if (!whole) {
+                                const uint32_t bits = at_bits(c_lo - c, c_hi - c);
 #pragma unroll
-                    for (int e = 0; e < 32; e++)
-                        if (!((bits >> e) & 1u)) v[e] = 0xff800000u;  // -infinity
-                }
+                                for (int e = 0; e < 32; e++)
+                                    if (!((bits >> e) & 1u)) v[e] = 0xff800000u;  // -infinity
+                            }
 #pragma unroll
-                for (int e = 0; e < 32; e += 4) {
-                    const ulonglong2 z = *reinterpret_cast<const ulonglong2*>(nl + c + e);
-                    float x0, x1, x2, x3;
-                    at_unpair(at_fma2(at_pair(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), sc2, z.x), x0, x1);
-                    at_unpair(at_fma2(at_pair(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])), sc2, z.y), x2, x3);
-                    sum[0] = at_add2(sum[0], at_pair(at_ex2(x0), at_ex2(x1)));
-                    sum[1] = at_add2(sum[1], at_pair(at_ex2(x2), at_ex2(x3)));
-                }
-            }
-            float u0, u1;
-            at_unpair(at_add2(sum[0], sum[1]), u0, u1);
-            total += u0 + u1;
-            __syncwarp();
-            if (lane == 0) at_arrive(&q_empty[st]);
-        }
-        part[tid] = total;
+                            for (int e = 0; e < 32; e += 4) {
+                                const ulonglong2 z = *reinterpret_cast<const ulonglong2*>(nl + c + e);
+                                float x0, x1, x2, x3;
+                                at_unpair(at_fma2(at_pair(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), sc2, z.x), x0, x1);
+                                at_unpair(at_fma2(at_pair(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])), sc2, z.y), x2, x3);
+                                sum[0] = at_add2(sum[0], at_pair(at_ex2(x0), at_ex2(x1)));
+                                sum[1] = at_add2(sum[1], at_pair(at_ex2(x2), at_ex2(x3)));
+                            }
+                        }
+                        float u0, u1;
+                        at_unpair(at_add2(sum[0], sum[1]), u0, u1);
+                        total += u0 + u1;
+                        __syncwarp();
+                        if (lane == 0) at_arrive(&q_empty[st]);
+                    }
     }
     if (!ok) at_flag(a.err, AT_ERR_WAIT);
+    cg::cluster_group cluster = cg::this_cluster();
+    if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    const int owners = min(split, WT_OWNERS), share = AT_N / owners;
+    if (warp < 4) (split > 1 ? cluster.map_shared_rank(part, tid / share) : part)[rank * share + tid % share] = total;
     // tensor memory back before the cluster's barrier
     at_before();
     __syncthreads();
     if (warp == 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(AT_N) : "memory");
-    cg::cluster_group cluster = cg::this_cluster();
-    if (split > 1) cluster.sync();
-    // position t of the tile is summed by rank t mod split
-    for (int t = rank + tid * split; t < AT_N; t += WT_THREADS * split) {
+    if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+    if (rank >= owners) return;
+    if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    for (int e = tid; e < share; e += WT_THREADS) {
+        const int t = rank * share + e;
         float w = 0.f;
-        for (int q = 0; q < split; q++) w += split > 1 ? *cluster.map_shared_rank(part + t, q) : part[t];
+        for (int q = 0; q < split; q++) w += part[q * share + e];
         const int j = j0 + t;
         if (j < len) {
             float* d = a.acc + seq * a.a_ss + kh * a.a_hs + j;
             *d = (j >= first ? 0.f : *d) + w;
         }
     }
-    if (split > 1) cluster.sync();  // the others may still be reading this CTA's sums
 }
 
 cudaError_t launch_attn_weights(const AttnOp& a, cudaStream_t s) {
