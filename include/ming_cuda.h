@@ -317,7 +317,8 @@ int ming_cuda_attn_decode(ming_ctx* ctx, const ming_kv_cache* cache, const ming_
  * holds min(len, keep) positions; lens is not written and to's is not read.
  * `to` may be `from` with acc_to = acc (in place); else the pages and totals
  * of the two do not overlap. A page shared by two sequences must not be
- * evicted in place. acc and acc_to may be NULL if keep = sinks + recent. */
+ * evicted in place. acc and acc_to may be NULL if keep = sinks + recent;
+ * otherwise keep is at most 49152. */
 typedef struct ming_evict {
     int keep, sinks, recent;
     const float* acc;

@@ -17,6 +17,7 @@ namespace ming {
 constexpr int AT_PAGE = 16;     // positions per page
 constexpr int AT_HD = 64;       // head dim
 constexpr int AT_MAXG = 8;      // query heads per kv head
+constexpr int AT_MAX_KEEP = 49152;  // positions an eviction by totals may leave (their list is in shared memory)
 constexpr float AT_LOG2E = 1.4426950408889634f;
 
 // Device error codes (the context's error word, read by ming_cuda_sync)

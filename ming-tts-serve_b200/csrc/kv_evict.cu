@@ -1,12 +1,18 @@
 // kv_evict.cu — eviction from a paged K/V cache by accumulated attention weight.
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "attn.cuh"
 
 namespace ming {
 
 namespace {
 constexpr int EV_THREADS = 256;
+constexpr int EV_WARPS = EV_THREADS / 32;
+constexpr int EV_BITS = 11;                 // radix of the selection: three digits of 11, 11 and 10 bits
+constexpr int EV_BINS = 1 << EV_BITS;
+constexpr int EV_AHEAD = 4;                 // 16-byte loads a thread has in flight
 
 // Order-preserving key of a total: larger total, larger key. -0 counts as +0
 // and NaN as -infinity.
@@ -15,126 +21,207 @@ MING_DEV uint32_t ev_key(float x) {
     const uint32_t u = __float_as_uint(x + 0.f);
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
+MING_DEV int ev_scan(int x, int lane) {  // inclusive
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    return x;
+}
 }  // namespace
 
-// One CTA per (sequence, layer, kv head). Which positions stay: the first
+// A cluster per (sequence, layer, kv head). Which positions stay: the first
 // `sinks`, the last `recent`, and of those between the keep - sinks - recent
-// of the largest total. The smallest total that stays is found digit by digit
-// (four passes of 8 bits over the keys, a histogram each); positions that tie
-// with it stay from the lowest on. Then the positions are walked in blocks of
-// EV_THREADS: the block's kept rows are read, and after a barrier written to
-// their places. A row's place is never behind it, so a block never overwrites
-// what a later one reads, and the move may be in place.
+// of the largest total. Its CTAs each find them for themselves (the totals are
+// a sixtieth of the rows' bytes and stay in the L1) and move a part of every
+// row each: K or V, and of it 128 / SPLIT bytes. Parts of a row do not meet, so
+// the move may be in place without a word between the CTAs; only the totals,
+// which all of them read, wait for the cluster before they are overwritten.
+//  * The smallest total that stays is found digit by digit: a histogram in
+//    shared memory, scanned from the top; the search ends early when a bin is
+//    taken whole. Positions that tie with it stay from the lowest on.
+//  * A warp counts its stretch of the positions, eight counts are summed, and
+//    the warp writes its kept positions to the list: two passes, one barrier.
+//  * Rows move EV_AHEAD x 256 x 16 bytes at a time, read before they are
+//    written. A row's place is never behind it, so what a batch writes no
+//    later one reads, and the next batch is read meanwhile.
+// Bound by the kept rows' bytes in a batch of sequences, by the chain of
+// dependent loads (length, totals, three histograms, pages, rows) for one.
+template <int SPLIT>
 __global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(const EvictOp a) {
-    __shared__ int hist[256];
-    __shared__ uint32_t s_prefix;
-    __shared__ int s_need, warp_kept[8], warp_ties[8], kept_pos[EV_THREADS];
-    const int b = blockIdx.z, layer = blockIdx.y, kh = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int seq = at_seq(a.from, b), n = at_len_of(a.from, seq, a.err), keep = min(a.keep, n);
-    const int lo = min(a.sinks, n), hi = max(lo, n - a.recent), need = n > a.keep ? a.keep - lo - (n - hi) : hi - lo;
+    extern __shared__ int ev_list[];  // positions that stay, ascending (when some between do and some do not)
+    __shared__ int hist[EV_BINS], warp_sum[EV_WARPS], warp_ties[EV_WARPS];
+    __shared__ int s_digit, s_left, s_bin;
+    constexpr int PARTS = 2 * SPLIT, LANES = 8 / SPLIT, ROWS = EV_THREADS / LANES;  // CTAs, lanes of a row, rows at once
+    const int part = blockIdx.x % PARTS, kh = blockIdx.x / PARTS, layer = blockIdx.y, b = blockIdx.z;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int seq = at_seq(a.from, b), n = at_len_of(a.from, seq, a.err), kept = min(a.keep, n);
+    const int lo = min(a.sinks, n), hi = max(lo, n - a.recent);
+    const int need = n > a.keep ? a.keep - lo - (n - hi) : hi - lo;  // of the positions [lo, hi) between
     const float* acc = a.acc ? a.acc + seq * a.a_ss + layer * a.a_ls + kh * a.a_hs : nullptr;
-    float* acc_to = a.acc_to ? a.acc_to + seq * a.t_ss + layer * a.t_ls + kh * a.t_hs : nullptr;
-    uint32_t cut = 0;   // positions between with a key above it stay
-    int ties = hi - lo; // and so many of those at it
-    if (need < hi - lo) {
-        if (need > 0) {
-            uint32_t prefix = 0;
-            int left = need;
-            for (int shift = 24; shift >= 0; shift -= 8) {
-                hist[tid] = 0;
-                __syncthreads();
-                for (int j = lo + tid; j < hi; j += EV_THREADS) {
-                    const uint32_t k = ev_key(acc[j]);
-                    if (shift == 24 || (k >> (shift + 8)) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
-                }
-                __syncthreads();
-                if (tid == 0) {
-                    int d = 255, above = 0;
-                    while (d > 0 && above + hist[d] < left) above += hist[d--];
-                    s_prefix = (prefix << 8) | (uint32_t)d;
-                    s_need = left - above;
-                }
-                __syncthreads();
-                prefix = s_prefix;
-                left = s_need;
-            }
-            cut = prefix;
-            ties = left;
-        } else {
-            cut = 0xffffffffu;
-            ties = 0;
-        }
-    }
-    const bool all = need >= hi - lo, none = need <= 0;
-    const int* bt = a.from.bt + (size_t)seq * a.from.bt_ld;
-    const int* bt_to = a.to.bt + (size_t)seq * a.to.bt_ld;
-    int slot0 = 0, ties0 = 0;  // kept, and ties seen, before this block
-    for (int j0 = 0; j0 < n; j0 += EV_THREADS) {
-        const int j = j0 + tid;
-        const bool mid = j >= lo && j < hi;
-        const uint32_t k = mid && !all && !none ? ev_key(acc[j]) : 0;
-        const bool tie = mid && !all && !none && k == cut;
-        const unsigned bt_tie = __ballot_sync(0xffffffffu, tie);
-        if (lane == 0) warp_ties[warp] = __popc(bt_tie);
-        __syncthreads();
-        int t = ties0 + __popc(bt_tie & ((1u << lane) - 1));
-        for (int w = 0; w < warp; w++) t += warp_ties[w];
-        const bool stays = j < n && (!mid || all || (!none && (k > cut || (tie && t < ties))));
-        const unsigned bs = __ballot_sync(0xffffffffu, stays);
-        if (lane == 0) warp_kept[warp] = __popc(bs);
-        __syncthreads();
-        int slot = __popc(bs & ((1u << lane) - 1)), total = 0;
-        for (int w = 0; w < 8; w++) {
-            if (w < warp) slot += warp_kept[w];
-            total += warp_kept[w];
-            ties0 += warp_ties[w];
-        }
-        if (stays) kept_pos[slot] = j;
-        const float av = stays && acc ? acc[j] : 0.f;
-        __syncthreads();
-        // the block's rows: K then V, eight 16-byte parts each
-        for (int which = 0; which < 2; which++) {
-            uint4 v[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int e = tid + i * EV_THREADS, s = e >> 3;
-                if (s < total) {
-                    const int p = kept_pos[s];
-                    const uint16_t* src = (which ? a.from.v : a.from.k) + layer * a.from_ls +
-                                          (int64_t)at_page(a.from, bt, p / AT_PAGE, a.err) * a.from.ps + kh * a.from.hs +
-                                          (p % AT_PAGE) * a.from.ss;
-                    v[i] = reinterpret_cast<const uint4*>(src)[e & 7];
-                }
+    const bool some = need > 0 && need < hi - lo;
+    if (some) {
+        // keys above `cut` stay, and the first `ties` of those at it; after an
+        // early end, every key from `cut` on
+        uint32_t cut = 0;
+        int ties = need, shift = 32;
+        for (int pass = 0; pass < 3; pass++) {
+            const int bits = pass < 2 ? EV_BITS : 10, above = shift;
+            shift -= bits;
+            for (int i = tid; i < EV_BINS; i += EV_THREADS) hist[i] = 0;
+            __syncthreads();
+            for (int j = lo + tid; j < hi; j += EV_THREADS) {
+                const uint32_t k = ev_key(acc[j]);
+                if (pass == 0 || (k >> above) == cut) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1);
             }
             __syncthreads();
+            // thread t holds bins from the top: the digit is where the sum reaches `ties`
+            constexpr int OWN = EV_BINS / EV_THREADS;
+            int mine = 0;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int e = tid + i * EV_THREADS, s = e >> 3;
-                if (s < total) {
-                    const int p = slot0 + s, page = bt_to[p / AT_PAGE];
-                    if ((unsigned)page < (unsigned)a.to.pages)
-                        reinterpret_cast<uint4*>((which ? a.to.v : a.to.k) + layer * a.to_ls + (int64_t)page * a.to.ps +
-                                                 kh * a.to.hs + (p % AT_PAGE) * a.to.ss)[e & 7] = v[i];
-                    else
-                        at_flag(a.err, AT_ERR_PAGE);
-                }
+            for (int i = 0; i < OWN; i++) mine += hist[EV_BINS - 1 - tid * OWN - i];
+            const int up_to = ev_scan(mine, lane);
+            if (lane == 31) warp_sum[warp] = up_to;
+            __syncthreads();
+            int before = up_to - mine;
+            for (int w = 0; w < warp; w++) before += warp_sum[w];
+            if (before < ties && before + mine >= ties) {
+                int i = EV_BINS - 1 - tid * OWN;
+                while (before + hist[i] < ties) before += hist[i--];
+                s_digit = i;
+                s_left = ties - before;
+                s_bin = hist[i];
             }
+            __syncthreads();
+            cut = (cut << bits) | (uint32_t)s_digit;
+            ties = s_left;
+            if (s_bin == ties) break;  // the bin stays whole
         }
-        if (stays) {
-            if (acc_to) acc_to[slot0 + slot] = av;
-            if (a.index) a.index[(((size_t)b * a.layers + layer) * a.kv_heads + kh) * a.keep + slot0 + slot] = j;
+        cut <<= shift;
+        const bool whole = s_bin == ties;  // keys >= cut stay
+        auto gt = [&](uint32_t k) { return whole ? k >= cut : k > cut; };
+        auto eq = [&](uint32_t k) { return !whole && k == cut; };
+        // a warp's stretch of [lo, hi), in whole warps
+        const int per = ((hi - lo + EV_THREADS - 1) / EV_THREADS) * 32;
+        const int w0 = min(hi, lo + warp * per), w1 = min(hi, w0 + per);
+        int gts = 0, eqs = 0;
+        for (int j = w0 + lane; j < w1; j += 32) {
+            const uint32_t k = ev_key(acc[j]);
+            gts += gt(k);
+            eqs += eq(k);
         }
-        slot0 += total;
+        gts = __reduce_add_sync(0xffffffffu, gts);
+        eqs = __reduce_add_sync(0xffffffffu, eqs);
+        __syncthreads();  // warp_sum's readers are done
+        if (lane == 0) {
+            warp_sum[warp] = gts;
+            warp_ties[warp] = eqs;
+        }
+        __syncthreads();
+        int at = lo, seen = 0;  // list place of the warp's first kept position; ties before it
+        for (int w = 0; w < warp; w++) {
+            at += warp_sum[w] + min(warp_ties[w], max(0, ties - seen));
+            seen += warp_ties[w];
+        }
+        for (int j = w0; j < w1; j += 32) {
+            const bool in = j + lane < w1;
+            const uint32_t k = in ? ev_key(acc[j + lane]) : 0;
+            const unsigned e = __ballot_sync(0xffffffffu, in && eq(k)), below = (1u << lane) - 1;
+            const bool stays = in && (gt(k) || (eq(k) && seen + __popc(e & below) < ties));
+            const unsigned s = __ballot_sync(0xffffffffu, stays);
+            if (stays) ev_list[at + __popc(s & below)] = j + lane;
+            at += __popc(s);
+            seen += __popc(e);
+        }
         __syncthreads();
     }
-    if (a.index)
-        for (int s = keep + tid; s < a.keep; s += EV_THREADS)
-            a.index[(((size_t)b * a.layers + layer) * a.kv_heads + kh) * a.keep + s] = -1;
+    // everyone has read the totals: they may be overwritten behind the matching wait
+    if (acc) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+    // the position that moves to place s
+    const int skipped = n - kept;
+    auto source = [&](int s) { return s < lo ? s : s >= kept - (n - hi) || !some ? s + (s < lo + need ? 0 : skipped) : ev_list[s]; };
+
+    const int* bt = a.from.bt + (size_t)seq * a.from.bt_ld;
+    const int* bt_to = a.to.bt + (size_t)seq * a.to.bt_ld;
+    const bool values = part >= SPLIT;
+    const uint16_t* src = (values ? a.from.v : a.from.k) + layer * a.from_ls + kh * a.from.hs;
+    uint16_t* dst = (values ? a.to.v : a.to.k) + layer * a.to_ls + kh * a.to.hs;
+    const int col = (part % SPLIT) * (AT_HD / SPLIT) + (tid % LANES) * 8, row = tid / LANES;
+    const bool in_place = src == dst && bt == bt_to;
+    auto read = [&](int s0, uint4 (&v)[EV_AHEAD]) {
+#pragma unroll
+        for (int i = 0; i < EV_AHEAD; i++) {
+            const int s = s0 + i * ROWS + row;
+            if (s >= kept) continue;
+            const int p = source(s);
+            v[i] = *reinterpret_cast<const uint4*>(src + (int64_t)at_page(a.from, bt, p / AT_PAGE, a.err) * a.from.ps +
+                                                   (p % AT_PAGE) * a.from.ss + col);
+        }
+    };
+    uint4 v[EV_AHEAD], w[EV_AHEAD];
+    // in place, the first places often are the positions themselves
+    int s0 = in_place ? lo / (EV_AHEAD * ROWS) * (EV_AHEAD * ROWS) : 0;
+    if (in_place && skipped == 0) s0 = kept;
+    if (s0 < kept) read(s0, v);
+    for (; s0 < kept; s0 += EV_AHEAD * ROWS) {
+        __syncthreads();  // the batch is read
+        const bool more = s0 + EV_AHEAD * ROWS < kept;
+        if (more) read(s0 + EV_AHEAD * ROWS, w);
+#pragma unroll
+        for (int i = 0; i < EV_AHEAD; i++) {
+            const int s = s0 + i * ROWS + row;
+            if (s >= kept) continue;
+            const int page = bt_to[s / AT_PAGE];
+            if ((unsigned)page < (unsigned)a.to.pages)
+                *reinterpret_cast<uint4*>(dst + (int64_t)page * a.to.ps + (s % AT_PAGE) * a.to.ss + col) = v[i];
+            else
+                at_flag(a.err, AT_ERR_PAGE);
+        }
+#pragma unroll
+        for (int i = 0; i < EV_AHEAD; i++) v[i] = w[i];
+    }
+    if (part == 0 && a.index) {
+        int* index = a.index + (((size_t)b * a.layers + layer) * a.kv_heads + kh) * a.keep;
+        for (int s = tid; s < a.keep; s += EV_THREADS) index[s] = s < kept ? source(s) : -1;
+    }
+    __syncwarp();
+    if (acc) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    if (acc && part == PARTS - 1) {
+        float* acc_to = a.acc_to + seq * a.t_ss + layer * a.t_ls + kh * a.t_hs;
+        for (int s = tid; s < (kept + EV_THREADS - 1) / EV_THREADS * EV_THREADS; s += EV_THREADS) {
+            const float x = s < kept ? acc[source(s)] : 0.f;
+            __syncthreads();  // as the rows: read, then written
+            if (s < kept) acc_to[s] = x;
+        }
+    }
 }
 
 cudaError_t launch_kv_evict(const EvictOp& a, cudaStream_t s) {
-    kv_evict_kernel<<<dim3(a.kv_heads, a.layers, a.seqs), EV_THREADS, 0, s>>>(a);
-    return cudaGetLastError();
+    static std::atomic<bool> ready[64] = {};  // per device: the kernels' attributes are set
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {
+        const void* f[2] = {(const void*)kv_evict_kernel<1>, (const void*)kv_evict_kernel<2>};
+        for (const void* k : f)
+            if ((e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, AT_MAX_KEEP * 4)) != cudaSuccess) return e;
+        if (dev < 64) ready[dev].store(true, std::memory_order_release);
+    }
+    const bool four = (long long)a.seqs * a.layers * a.kv_heads * 2 < 2 * 148;  // few heads: four CTAs each, half rows
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.kv_heads * (four ? 4 : 2), a.layers, a.seqs);
+    cfg.blockDim = dim3(EV_THREADS);
+    cfg.dynamicSmemBytes = a.sinks + a.recent < a.keep ? (size_t)a.keep * 4 : 0;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = four ? 4 : 2;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return four ? cudaLaunchKernelEx(&cfg, kv_evict_kernel<2>, a) : cudaLaunchKernelEx(&cfg, kv_evict_kernel<1>, a);
 }
 
 }  // namespace ming

@@ -112,7 +112,7 @@ def test_null_structures():
     (dict(), dict(sinks=20, recent=13), "fit in keep"), (dict(), dict(sinks=2**31 - 1, recent=2**31 - 1), "fit in keep"),
     (dict(bt_ld=1, max_len=16), dict(), "does not fit to's"), (dict(), dict(acc=0, acc_to=0), "acc is null"),
     (dict(), dict(acc_to=0), "go together"), (dict(), dict(acc=0, sinks=24), "go together"), (dict(), dict(index=AT + 2), "4-byte"),
-    (dict(), dict(acc_to_seq_stride=-1), "negative"), (dict(), dict(acc_to=AT, acc_to_head_stride=64), "other strides"),
+    (dict(bt_ld=9999, max_len=159984), dict(keep=49153), "at most 49152"), (dict(), dict(acc_to_seq_stride=-1), "negative"), (dict(), dict(acc_to=AT, acc_to_head_stride=64), "other strides"),
 ])
 def test_evict_arguments(to, bad, word):
     _ensure_built()
