@@ -14,12 +14,10 @@ namespace ming {
 namespace {
 namespace cg = cooperative_groups;
 
-constexpr int DE_WARPS = 8;
-constexpr int DE_THREADS = DE_WARPS * 32;
-constexpr int DE_MAX_SPLIT = 16;  // CTAs of a cluster
-constexpr int DE_OLD = AT_HD + 4;                                 // row of merged outputs: float4-aligned, rows on other banks
-constexpr int DE_PART = DE_WARPS * AT_MAXG * (DE_OLD + 2);        // floats: every warp's outputs, maxima and sums
-constexpr int DE_SMEM = (DE_PART + AT_MAXG * (DE_OLD + 2) + 2 * AT_MAXG) * 4;
+constexpr int DE_MAX_SPLIT = 16;          // CTAs of a cluster
+constexpr int DE_OLD = AT_HD + 4;         // row of merged outputs: float4-aligned, rows on other banks
+constexpr int de_part(int warps) { return warps * AT_MAXG * (DE_OLD + 2); }  // floats: every warp's outputs, maxima and sums
+constexpr int de_smem(int warps) { return (de_part(warps) + AT_MAXG * (DE_OLD + 2) + 2 * AT_MAXG) * 4; }
 constexpr int DE_SMEM_MAX = 200 * 1024;
 
 enum { DE_PLAIN = 0, DE_TRACK = 1, DE_TRACK_AGAIN = 2 };
@@ -67,13 +65,14 @@ MING_DEV uint32_t de_prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_
 // (longer than fits) reads the keys a second time.
 // Bound by: the cache's bytes (256 per position and kv head) for batches, the
 // launch, two dependent loads and the cluster's two barriers for short rows.
-template <int MODE>
-__global__ void __launch_bounds__(DE_THREADS, 2) attn_decode_kernel(const AttnOp a, int sc_ld) {
-    extern __shared__ __align__(16) float de_smem[];
-    float* wo = de_smem;                                 // [warp][head][DE_OLD]
-    float* wm = wo + DE_WARPS * AT_MAXG * DE_OLD;        // [warp][head]
-    float* wl = wm + DE_WARPS * AT_MAXG;
-    float* co = de_smem + DE_PART;                       // this CTA's [head][DE_OLD], unnormalised
+template <int MODE, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) attn_decode_kernel(const AttnOp a, int sc_ld) {
+    constexpr int THREADS = WARPS * 32;
+    extern __shared__ __align__(16) float de_buf[];
+    float* wo = de_buf;                                  // [warp][head][DE_OLD]
+    float* wm = wo + WARPS * AT_MAXG * DE_OLD;        // [warp][head]
+    float* wl = wm + WARPS * AT_MAXG;
+    float* co = de_buf + de_part(WARPS);                       // this CTA's [head][DE_OLD], unnormalised
     float* cm = co + AT_MAXG * DE_OLD;
     float* cl = cm + AT_MAXG;
     float* fm = cl + AT_MAXG;                            // the cluster's maxima and 1 / sums
@@ -100,11 +99,11 @@ __global__ void __launch_bounds__(DE_THREADS, 2) attn_decode_kernel(const AttnOp
     for (int i = 0; i < 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 
     // this warp's pages: v0 + warp, + 8, ..; a lane looks up every 32nd ahead of use
-    const int first = v0 + warp, count = first < v1 ? (v1 - first + DE_WARPS - 1) / DE_WARPS : 0;
+    const int first = v0 + warp, count = first < v1 ? (v1 - first + WARPS - 1) / WARPS : 0;
     int ids = 0;
     auto look_up = [&](int i0) {
         const int i = i0 + lane;
-        ids = i < count ? at_page(a.kv, bt, see.page(first + i * DE_WARPS), a.err) : 0;
+        ids = i < count ? at_page(a.kv, bt, see.page(first + i * WARPS), a.err) : 0;
     };
     uint4 kf[4], vf[4];  // the page in flight
     auto fetch_k = [&](int64_t base) {
@@ -151,7 +150,7 @@ __global__ void __launch_bounds__(DE_THREADS, 2) attn_decode_kernel(const AttnOp
         fetch_v(base);
     }
     for (int i = 0; i < count; i++) {
-        const int vi = first + i * DE_WARPS, p = see.page(vi);
+        const int vi = first + i * WARPS, p = see.page(vi);
         uint4 k[4] = {kf[0], kf[1], kf[2], kf[3]}, v[4] = {vf[0], vf[1], vf[2], vf[3]};
         if (i + 1 < count) {
             if (((i + 1) & 31) == 0) look_up(i + 1);
@@ -215,28 +214,42 @@ __global__ void __launch_bounds__(DE_THREADS, 2) attn_decode_kernel(const AttnOp
                                                                         o[d + 2][c] + o[d + 2][c + 2], o[d + 3][c] + o[d + 3][c + 2]);
     }
     __syncthreads();
-    // the CTA's part: warp h joins head h, two dims a lane
+    // the CTA's part: eight warps a head each, or sixteen half a head
     {
-        const int h = warp;
-        float M = -INFINITY, L = 0.f, x = 0.f, y = 0.f;
+        constexpr int DIMS = 16 / WARPS;  // a lane's
+        const int h = warp % AT_MAXG, d0 = (warp / AT_MAXG) * 32 + DIMS * lane;
+        float M = -INFINITY, L = 0.f, x[DIMS] = {};
 #pragma unroll
-        for (int w = 0; w < DE_WARPS; w++) M = fmaxf(M, wm[w * AT_MAXG + h]);
+        for (int w = 0; w < WARPS; w++) M = fmaxf(M, wm[w * AT_MAXG + h]);
 #pragma unroll
-        for (int w = 0; w < DE_WARPS; w++) {
+        for (int w = 0; w < WARPS; w++) {
             const float f = M == -INFINITY ? 0.f : exp2f(wm[w * AT_MAXG + h] - M);
-            const float2 v = *reinterpret_cast<const float2*>(wo + (w * AT_MAXG + h) * DE_OLD + 2 * lane);
             L += wl[w * AT_MAXG + h] * f;
-            x += v.x * f;
-            y += v.y * f;
+#pragma unroll
+            for (int d = 0; d < DIMS; d++) x[d] += wo[(w * AT_MAXG + h) * DE_OLD + d0 + d] * f;
         }
-        *reinterpret_cast<float2*>(co + h * DE_OLD + 2 * lane) = make_float2(x, y);
-        if (lane == 0) cm[h] = M, cl[h] = L;
+#pragma unroll
+        for (int d = 0; d < DIMS; d++) co[h * DE_OLD + d0 + d] = x[d];
+        if (lane == 0 && warp < AT_MAXG) cm[h] = M, cl[h] = L;
     }
+    // the totals that this thread adds to, on their way while the parts meet
+    float* const acc = MODE == DE_TRACK ? a.acc + seq * a.a_ss + kh * a.a_hs : nullptr;
+    const int mine = (v1 - v0) * AT_PAGE;
+    float old[4];
+    auto position = [&](int e) { return see.page(v0 + e / AT_PAGE) * AT_PAGE + e % AT_PAGE; };
+    auto fetch_acc = [&](int e0) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int e = e0 + k * THREADS, j = e < mine ? position(e) : see.n;
+            old[k] = see.sees(j) && j != see.n - 1 ? acc[j] : 0.f;
+        }
+    };
+    if (MODE == DE_TRACK) fetch_acc(tid);
     cg::cluster_group cluster = cg::this_cluster();
     if (ns > 1) cluster.sync();
     else __syncthreads();
     // the cluster's: the group's outputs, two dims at a time, over the ranks
-    for (int e = rank * DE_THREADS + tid; e < a.group * (AT_HD / 2); e += ns * DE_THREADS) {
+    for (int e = rank * THREADS + tid; e < a.group * (AT_HD / 2); e += ns * THREADS) {
         const int h = e / (AT_HD / 2), d = e % (AT_HD / 2);
         float M = -INFINITY, L = 0.f, x = 0.f, y = 0.f;
         for (int r = 0; r < ns; r++) M = fmaxf(M, ns > 1 ? *cluster.map_shared_rank(cm + h, r) : cm[h]);
@@ -263,21 +276,30 @@ __global__ void __launch_bounds__(DE_THREADS, 2) attn_decode_kernel(const AttnOp
             fl[tid] = L > 0.f ? 1.f / L : 0.f;
         }
         __syncthreads();
-        float* acc = a.acc + seq * a.a_ss + kh * a.a_hs;
         if (MODE == DE_TRACK) {
-            for (int e = tid; e < (v1 - v0) * AT_PAGE; e += DE_THREADS) {
-                const int j = see.page(v0 + e / AT_PAGE) * AT_PAGE + e % AT_PAGE;
-                if (!see.sees(j)) continue;
-                float w = 0.f;
-                for (int h = 0; h < a.group; h++) w += exp2f(sc[h * sc_ld + e] - fm[h]) * fl[h];
-                acc[j] = (j == see.n - 1 ? 0.f : acc[j]) + w;
+            for (int e0 = tid; e0 < mine; e0 += 4 * THREADS) {
+                float now[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int e = e0 + k * THREADS;
+                    float w = 0.f;
+                    if (e < mine)
+                        for (int h = 0; h < a.group; h++) w += exp2f(sc[h * sc_ld + e] - fm[h]) * fl[h];
+                    now[k] = old[k] + w;
+                }
+                fetch_acc(e0 + 4 * THREADS);
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int e = e0 + k * THREADS, j = e < mine ? position(e) : see.n;
+                    if (see.sees(j)) acc[j] = now[k];
+                }
             }
         } else {
             const float M = fm[g], il = g < a.group ? fl[g] : 0.f;
             look_up(0);
             for (int i = 0; i < count; i++) {
                 if (i > 0 && (i & 31) == 0) look_up(i);
-                const int p = see.page(first + i * DE_WARPS);
+                const int p = see.page(first + i * WARPS);
                 fetch_k(base_of(i));
                 float c[4];
                 logits(kf, p, c);
@@ -287,7 +309,8 @@ __global__ void __launch_bounds__(DE_THREADS, 2) attn_decode_kernel(const AttnOp
 #pragma unroll
                     for (int s = 4; s < 32; s <<= 1) w += __shfl_xor_sync(0xffffffffu, w, s);
                     const int j = p * AT_PAGE + 2 * t + (d & 1) + 4 * (d & 2);
-                    if (g == 0 && see.sees(j)) acc[j] = (j == see.n - 1 ? 0.f : acc[j]) + w;
+                    float* total = a.acc + seq * a.a_ss + kh * a.a_hs + j;
+                    if (g == 0 && see.sees(j)) *total = (j == see.n - 1 ? 0.f : *total) + w;
                 }
             }
         }
@@ -301,8 +324,9 @@ cudaError_t launch_attn_decode(const AttnOp& a, cudaStream_t s) {
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {
-        const void* f[3] = {(const void*)attn_decode_kernel<DE_PLAIN>, (const void*)attn_decode_kernel<DE_TRACK>,
-                            (const void*)attn_decode_kernel<DE_TRACK_AGAIN>};
+        const void* f[6] = {(const void*)attn_decode_kernel<DE_PLAIN, 8>,       (const void*)attn_decode_kernel<DE_TRACK, 8>,
+                            (const void*)attn_decode_kernel<DE_TRACK_AGAIN, 8>, (const void*)attn_decode_kernel<DE_PLAIN, 16>,
+                            (const void*)attn_decode_kernel<DE_TRACK, 16>,      (const void*)attn_decode_kernel<DE_TRACK_AGAIN, 16>};
         for (const void* k : f) {
             if ((e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, DE_SMEM_MAX)) != cudaSuccess) return e;
             if ((e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
@@ -315,14 +339,20 @@ cudaError_t launch_attn_decode(const AttnOp& a, cudaStream_t s) {
         a.window ? std::min(most, ((long long)a.window + 2 * AT_PAGE - 2) / AT_PAGE +
                                       std::min(most, ((long long)a.sinks + AT_PAGE - 1) / AT_PAGE))
                  : most;
-    // splits: two CTAs for every SM if there are pages enough to give each warp one
+    // Splits: as many as fill the SMs once, two CTAs each, if there are pages
+    // enough to give each warp one. (64 x 4096 positions, 128 heads: 42 us in
+    // one part, 29 in two, 34 in four, 46 in eight.) Where that leaves SMs
+    // with one CTA or none, CTAs of sixteen warps keep more loads in flight
+    // (one cache of 32768 positions: 21 us with eight, 14 with sixteen).
+    const long long heads = (long long)a.seqs * a.kv_heads;
     int ns = 1;
-    while (ns < DE_MAX_SPLIT && (long long)a.seqs * a.kv_heads * ns < 2 * 148 && pages >= 2 * ns * DE_WARPS) ns *= 2;
+    while (ns < DE_MAX_SPLIT && heads * ns * 2 <= 2 * 148 && pages >= 2 * ns * 8) ns *= 2;
+    const int warps = heads * ns <= 148 && pages >= 2 * 16 * ns ? 16 : 8;
     int mode = DE_PLAIN, ld = 0;
-    size_t smem = DE_SMEM;
+    size_t smem = de_smem(warps);
     if (a.acc) {
         const long long per = (pages + ns - 1) / ns * AT_PAGE;
-        const size_t want = DE_SMEM + (size_t)(per / 32 * 32 + 40) * AT_MAXG * 4;
+        const size_t want = smem + (size_t)(per / 32 * 32 + 40) * AT_MAXG * 4;
         mode = want <= DE_SMEM_MAX ? DE_TRACK : DE_TRACK_AGAIN;
         if (mode == DE_TRACK) {
             smem = want;
@@ -331,7 +361,7 @@ cudaError_t launch_attn_decode(const AttnOp& a, cudaStream_t s) {
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ns, a.kv_heads, a.seqs);
-    cfg.blockDim = dim3(DE_THREADS);
+    cfg.blockDim = dim3(warps * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
@@ -341,9 +371,11 @@ cudaError_t launch_attn_decode(const AttnOp& a, cudaStream_t s) {
     at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    if (mode == DE_PLAIN) return cudaLaunchKernelEx(&cfg, attn_decode_kernel<DE_PLAIN>, a, ld);
-    if (mode == DE_TRACK) return cudaLaunchKernelEx(&cfg, attn_decode_kernel<DE_TRACK>, a, ld);
-    return cudaLaunchKernelEx(&cfg, attn_decode_kernel<DE_TRACK_AGAIN>, a, ld);
+    using Kernel = void (*)(AttnOp, int);
+    static const Kernel kernels[2][3] = {
+        {attn_decode_kernel<DE_PLAIN, 8>, attn_decode_kernel<DE_TRACK, 8>, attn_decode_kernel<DE_TRACK_AGAIN, 8>},
+        {attn_decode_kernel<DE_PLAIN, 16>, attn_decode_kernel<DE_TRACK, 16>, attn_decode_kernel<DE_TRACK_AGAIN, 16>}};
+    return cudaLaunchKernelEx(&cfg, kernels[warps == 16][mode], a, ld);
 }
 
 }  // namespace ming

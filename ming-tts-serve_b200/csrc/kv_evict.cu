@@ -8,11 +8,11 @@
 namespace ming {
 
 namespace {
-constexpr int EV_THREADS = 256;
+constexpr int EV_THREADS = 512;
 constexpr int EV_WARPS = EV_THREADS / 32;
 constexpr int EV_BITS = 11;                 // radix of the selection: three digits of 11, 11 and 10 bits
 constexpr int EV_BINS = 1 << EV_BITS;
-constexpr int EV_AHEAD = 4;                 // 16-byte loads a thread has in flight
+constexpr int EV_AHEAD = 2;                 // 16-byte loads a thread has in flight
 
 // Order-preserving key of a total: larger total, larger key. -0 counts as +0
 // and NaN as -infinity.
@@ -49,7 +49,7 @@ MING_DEV int ev_scan(int x, int lane) {  // inclusive
 // Bound by the kept rows' bytes in a batch of sequences, by the chain of
 // dependent loads (length, totals, three histograms, pages, rows) for one.
 template <int SPLIT>
-__global__ void __launch_bounds__(EV_THREADS) kv_evict_kernel(const EvictOp a) {
+__global__ void __launch_bounds__(EV_THREADS, 4) kv_evict_kernel(const EvictOp a) {
     extern __shared__ int ev_list[];  // positions that stay, ascending (when some between do and some do not)
     __shared__ int hist[EV_BINS], warp_sum[EV_WARPS], warp_ties[EV_WARPS];
     __shared__ int s_digit, s_left, s_bin;
