@@ -341,22 +341,29 @@ cudaError_t launch_attn_decode(const AttnOp& a, cudaStream_t s) {
                  : most;
     // Splits: as many as fill the SMs once, two CTAs each, if there are pages
     // enough to give each warp one. (64 x 4096 positions, 128 heads: 42 us in
-    // one part, 29 in two, 34 in four, 46 in eight.) Where that leaves SMs
-    // with one CTA or none, CTAs of sixteen warps keep more loads in flight
-    // (one cache of 32768 positions: 21 us with eight, 14 with sixteen).
+    // one part, 29 in two, 34 in four, 46 in eight.) Clusters of sixteen find
+    // place one at a time in each part of the chip: for few heads alone (8 x
+    // 4096, 16 heads: 10.4 us in eight parts, 16.5 in sixteen; 1 x 4096: 8.6
+    // and 7.6). Sixteen warps a CTA pay on a cache that gives each warp four
+    // pages (1 x 32768: 15.8 us against 18.9; 1 x 2048: 7.3 against 6.5).
     const long long heads = (long long)a.seqs * a.kv_heads;
     int ns = 1;
-    while (ns < DE_MAX_SPLIT && heads * ns * 2 <= 2 * 148 && pages >= 2 * ns * 8) ns *= 2;
-    const int warps = heads * ns <= 148 && pages >= 2 * 16 * ns ? 16 : 8;
+    while (ns < DE_MAX_SPLIT && heads * ns * 2 <= (ns == 8 ? 64 : 2 * 148) && pages >= 2 * ns * 8) ns *= 2;
+    const int warps = heads * ns <= 64 && pages >= 4 * 16 * ns ? 16 : 8;
+    auto ld_of = [&](int ns) {  // 8 past a multiple of 32: the eight heads' stores fall on distinct banks
+        return (pages + ns - 1) / ns * AT_PAGE / 32 * 32 + 40;
+    };
+    auto track = [&](int ns) { return de_smem(warps) + ld_of(ns) * AT_MAXG * 4; };
     int mode = DE_PLAIN, ld = 0;
     size_t smem = de_smem(warps);
     if (a.acc) {
-        const long long per = (pages + ns - 1) / ns * AT_PAGE;
-        const size_t want = smem + (size_t)(per / 32 * 32 + 40) * AT_MAXG * 4;
-        mode = want <= DE_SMEM_MAX ? DE_TRACK : DE_TRACK_AGAIN;
+        // logits leave the L1 room for the loads in flight: with 86 KB of them
+        // a CTA (two parts) 64 x 4096 positions took 41.5 us, with 53 KB 38.4
+        while (ns < 8 && heads * ns > 148 && track(ns) > 56 * 1024) ns *= 2;
+        mode = track(ns) <= DE_SMEM_MAX ? DE_TRACK : DE_TRACK_AGAIN;
         if (mode == DE_TRACK) {
-            smem = want;
-            ld = (int)(per / 32 * 32 + 40);  // 8 past a multiple of 32: the eight heads' stores fall on distinct banks
+            smem = track(ns);
+            ld = (int)ld_of(ns);
         }
     }
     cudaLaunchConfig_t cfg = {};
