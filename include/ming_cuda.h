@@ -66,6 +66,13 @@ typedef struct ming_cfg {
      * upsampled x4, an ISTFT head (n_fft 3528, hop 882) */
     int vae_layers, vae_ff, vae_window;
     int vae_max_latents; /* latents per ming_cuda_vae_decode call */
+    /* LM attention over bounded caches (0 / 0 / 0: every position is seen and
+     * kept, the reference's behaviour). attn_window > 0: a row sees the last
+     * attn_window positions of its sequence's cache, itself among them, and
+     * the first attn_sinks. kv_track: the weights that attention gives to
+     * each cached position are added up per (sequence, layer, kv head), for
+     * ming_cuda_seq_evict (4 bytes per position, layer and kv head). */
+    int attn_window, attn_sinks, kv_track;
 } ming_cfg;
 
 void ming_cuda_default_cfg(ming_cfg* cfg);
@@ -104,6 +111,19 @@ int ming_cuda_seq_len(ming_ctx* ctx, int seq_id, int* len);
 /* Truncates a sequence to `len` positions (pages are kept for reuse). */
 int ming_cuda_seq_truncate(ming_ctx* ctx, int seq_id, int len);
 
+/* Brings a sequence of a context with attn_window or kv_track back to `keep`
+ * cached positions if it holds more: in every layer and kv head the first
+ * `sinks`, the last `recent` and, of those between, the ones of the largest
+ * attention totals stay (ming_cuda_kv_evict's rule; without kv_track, keep
+ * must be sinks + recent). They move together in order, pages behind them
+ * return to the pool, and seq_len is `keep` afterwards. Keys stay as they
+ * were rotated, and the next position's rotation goes on from the number of
+ * positions that the sequence has seen in all. attn_window and attn_sinks
+ * count positions of the cache as it is then. Asynchronous. No reference
+ * counterpart (the reference ends a sequence at 512 positions,
+ * src/ming_model.zig:46-47). */
+int ming_cuda_seq_evict(ming_ctx* ctx, int seq_id, int keep, int sinks, int recent);
+
 /* Model.lmForward for a multi-row prompt (QStack.forward with L > 1,
  * src/ming_model.zig:566-614): x [L][hidden] at positions len..len+L-1,
  * appends K/V. out [L][hidden] post-norm hidden (may be NULL), stop [L]
@@ -132,7 +152,7 @@ int ming_cuda_lm_generate(ming_ctx* ctx, int B, const int* seq_ids, const uint16
  * fixed 4 MiB array compiled into the library (held by every GPU that loads
  * the library until the process exits). A step needing more than that
  * (B x ceil(max_ctx / 256) x heads x 264 bytes) is rejected with
- * MING_ERR_INVALID. The first call on a device looks up the array's device
+ * MING_ERR_INVALID, as is a context with attn_window or kv_track. The first call on a device looks up the array's device
  * address; make that first call before any stream capture. All calls on a
  * device share the array and its contents persist between calls; nothing in
  * it needs to start at zero, but calls that overlap on the GPU (other
@@ -354,6 +374,9 @@ int ming_cuda_kv_read(ming_ctx* ctx, int seq_id, int layer, int pos0, int n, uin
  * No reference counterpart (the reference's KvCache holds MLX arrays,
  * src/ming_model.zig:638-662). */
 int ming_cuda_kv_write(ming_ctx* ctx, int seq_id, int layer, int pos0, int n, const uint16_t* k, const uint16_t* v);
+/* Attention totals of positions [pos0, pos0+n) of one layer (kv_track): out
+ * host [kv_heads][n] f32. Positions written by ming_cuda_kv_write start at 0. */
+int ming_cuda_kv_totals(ming_ctx* ctx, int seq_id, int layer, int pos0, int n, float* out);
 /* Dequantizes a loaded linear back from its device tiles (the kernels' own
  * unpack path): out host [out][in] f32 in the reference's row order. */
 int ming_cuda_unpack_linear(ming_ctx* ctx, const char* weight_name, float* out);

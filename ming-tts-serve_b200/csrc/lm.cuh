@@ -40,6 +40,9 @@ MING_DEV size_t kv_index(const KvDev& kv, int page, int layer, int which, int h,
 struct RowsDev {
     const int* seq;
     const int* pos;
+    // [max_seqs] or null: positions evicted from a sequence's cache, which its
+    // rows' rotations go on counting
+    const int* shift = nullptr;
 };
 
 // Tile layout of the fused q|k|v linear: tile t covers head t/4 of its block,
@@ -58,10 +61,10 @@ struct EpiQKV {
         const int h = lt >> 2, d = (lt & 3) * 8 + r8;
         float x1 = rb(lo + bias[tile * 16 + r8]);
         float x2 = rb(hi + bias[tile * 16 + r8 + 8]);
-        const int pos = rows.pos[row], seq = which ? rows.seq[row] : 0;
+        const int pos = rows.pos[row], seq = which || rows.shift ? rows.seq[row] : 0;
         if (which < 2) {
             // MLX fast_rope (non-traditional): angle = pos * 2^(-(d/32) log2 theta), f32
-            const float th = (float)pos * exp2f(-((float)d / 32.0f) * log2_theta);
+            const float th = (float)(rows.shift ? pos + rows.shift[seq] : pos) * exp2f(-((float)d / 32.0f) * log2_theta);
             float s, c;
             sincosf(th, &s, &c);
             const float a = x1 * c - x2 * s, b = x1 * s + x2 * c;

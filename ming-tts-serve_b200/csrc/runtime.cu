@@ -374,25 +374,79 @@ long long* ktrace_slot(ming_ctx* c) {
     return c->ktrace + (size_t)(c->ktrace_used++) * KT_CTAS * 8;
 }
 
+// The attention of one layer over a bounded cache: `rows` decode rows, or the
+// prefill chunk that pf_seq and pf_meta describe.
+cudaError_t enqueue_bounded_attn(ming_ctx* c, int layer, int rows, bool decode) {
+    const ming_cfg& f = c->cfg;
+    AttnOp a{};
+    a.kv.ps = (int64_t)f.layers * 2 * f.kv_heads * PAGE * HD;
+    a.kv.hs = PAGE * HD;
+    a.kv.ss = HD;
+    a.kv.k = c->pool + (int64_t)layer * 2 * f.kv_heads * PAGE * HD;
+    a.kv.v = a.kv.k + (int64_t)f.kv_heads * PAGE * HD;
+    a.kv.bt_ld = c->bt_ld;
+    a.kv.pages = f.max_pages;
+    a.kv.max_len = f.max_ctx;
+    a.q = c->q;
+    a.out = c->att;
+    a.q_rs = a.o_rs = f.heads * HD;
+    a.q_hs = a.o_hs = HD;
+    a.heads = f.heads;
+    a.kv_heads = f.kv_heads;
+    a.group = f.heads / f.kv_heads;
+    a.window = f.attn_window;
+    a.sinks = f.attn_sinks;
+    a.scale_log2 = 0.125f * AT_LOG2E;
+    a.a_ss = (int64_t)f.layers * f.kv_heads * f.max_ctx;
+    a.a_hs = f.max_ctx;
+    float* acc = c->kv_acc ? c->kv_acc + (int64_t)layer * f.kv_heads * f.max_ctx : nullptr;
+    a.rows = a.max_rows = rows;
+    a.err = c->dev_err;
+    if (decode) {
+        a.kv.bt = c->bt;
+        a.kv.lens = c->seq_len;
+        a.kv.seq_ids = c->row_seq;
+        a.kv.len_add = 1;  // the step's own position is counted at its end
+        a.seqs = rows;
+        a.max_rows = 1;
+        a.acc = acc;
+        return launch_attn_decode(a, c->stream);
+    }
+    a.kv.bt = c->bt + (size_t)c->pf_seq * c->bt_ld;
+    a.kv.lens = c->pf_meta + 2;
+    a.q_start = c->pf_meta;
+    a.seqs = 1;
+    a.lse = c->lse;
+    cudaError_t e = launch_attn_prefill(a, c->stream);
+    if (e != cudaSuccess || !acc) return e;
+    a.acc = acc + (int64_t)c->pf_seq * a.a_ss;
+    return launch_attn_weights(a, c->stream);
+}
+
 // The 24-layer step over `rows` rows whose row_seq/row_pos are on the device.
 // Returns the first failed attention launch (the linears' launches are
 // checked by the caller's cudaGetLastError).
 cudaError_t enqueue_layers(ming_ctx* c, int rows, bool decode) {
     const ming_cfg& f = c->cfg;
     c->ktrace_used = 0;
-    RowsDev rd{c->row_seq, c->row_pos};
+    RowsDev rd{c->row_seq, c->row_pos, c->seq_shift};
     KvDev kv{c->pool, c->bt, c->bt_ld, f.layers, f.kv_heads};
     for (int l = 0; l < f.layers; l++) {
         auto& L = c->layers[l];
         run_linear(c, L.qkv.w, ProRms{c->x, L.ln1, f.hidden, f.hidden, f.rms_eps, 0, nullptr, L.ln1_unit},
                    EpiQKV{L.qkv.w.bias, c->q, kv, rd, l, f.heads, f.kv_heads, c->log2_theta}, rows, c->stream);
-        AttnArgs aa{c->q, c->part, kv, rd, l, f.heads, f.kv_heads, c->nsplit, decode ? 1 : 0, c->att};
-        aa.tmap = &c->kv_tmap;
-        aa.err = c->dev_err;
-        aa.trace = (long)aa.nsplit_max * aa.kv_heads * rows <= KT_CTAS ? ktrace_slot(c) : nullptr;
-        cudaError_t e = launch_attn(aa, rows, c->stream);
-        if (e == cudaSuccess && !attn_fused_combine(aa))
-            e = launch_attn_combine(c->part, rd, c->nsplit, f.heads, c->att, rows, c->stream);
+        cudaError_t e = cudaSuccess;
+        if (c->bounded) {
+            e = enqueue_bounded_attn(c, l, rows, decode);
+        } else {
+            AttnArgs aa{c->q, c->part, kv, rd, l, f.heads, f.kv_heads, c->nsplit, decode ? 1 : 0, c->att};
+            aa.tmap = &c->kv_tmap;
+            aa.err = c->dev_err;
+            aa.trace = (long)aa.nsplit_max * aa.kv_heads * rows <= KT_CTAS ? ktrace_slot(c) : nullptr;
+            e = launch_attn(aa, rows, c->stream);
+            if (e == cudaSuccess && !attn_fused_combine(aa))
+                e = launch_attn_combine(c->part, rd, c->nsplit, f.heads, c->att, rows, c->stream);
+        }
         if (e != cudaSuccess) return e;
         run_linear(c, L.o.w, ProPlain{c->att, f.heads * HD, 0},
                    EpiResidual{c->x, c->x1, nullptr, f.hidden}, rows, c->stream);
@@ -829,6 +883,9 @@ void ming_cuda_default_cfg(ming_cfg* c) {
     c->vae_ff = 4864;
     c->vae_window = 64;
     c->vae_max_latents = 512;
+    c->attn_window = 0;
+    c->attn_sinks = 0;
+    c->kv_track = 0;
 }
 
 int ming_cuda_create(int device, const ming_cfg* cfg, ming_ctx** out) {
@@ -842,6 +899,9 @@ int ming_cuda_create(int device, const ming_cfg* cfg, ming_ctx** out) {
         return fail(MING_ERR_INVALID, "heads must be a multiple of kv_heads with at most 8 per group");
     if (f.group_size != 64) return fail(MING_ERR_INVALID, "group_size must be 64");
     if (f.max_ctx < PAGE || f.max_ctx % ATT_SPLIT) return fail(MING_ERR_INVALID, "max_ctx must be a multiple of 256");
+    if (f.attn_window < 0 || f.attn_sinks < 0 || (f.attn_sinks && !f.attn_window))
+        return fail(MING_ERR_INVALID, "attn_window and attn_sinks must not be negative, sinks need a window");
+    if (f.kv_track != 0 && f.kv_track != 1) return fail(MING_ERR_INVALID, "kv_track must be 0 or 1");
     if (f.max_batch < 1 || f.max_batch > 256 || f.max_prefill < 1 || f.max_seqs < 1 || f.max_pages < 1)
         return fail(MING_ERR_INVALID, "bad batch/prefill/sequence/page limits");
     if (f.dit_mode != MING_DIT_NONE) {
@@ -859,6 +919,7 @@ int ming_cuda_create(int device, const ming_cfg* cfg, ming_ctx** out) {
     std::unique_ptr<ming_ctx> c(new ming_ctx());
     c->device = device;
     c->cfg = f;
+    c->bounded = f.attn_window > 0 || f.kv_track;
     CK(cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking));
     int rc = MING_OK;
     c->dev_err = c->mem.alloc<int>(1, &rc);
@@ -965,6 +1026,14 @@ int ming_cuda_finalize(ming_ctx* c) {
     c->row_seq = c->mem.alloc<int>(c->maxr, &rc);
     c->row_pos = c->mem.alloc<int>(c->maxr, &rc);
     c->step_counter = c->mem.alloc<int>(2, &rc);
+    if (c->bounded) {
+        c->seq_shift = c->mem.alloc<int>(f.max_seqs, &rc);
+        c->pf_meta = c->mem.alloc<int>(3, &rc);
+        if (f.kv_track) {
+            c->kv_acc = c->mem.alloc<float>((size_t)f.max_seqs * f.layers * f.kv_heads * f.max_ctx, &rc);
+            c->lse = c->mem.alloc<float>((size_t)c->maxr * f.heads, &rc);
+        }
+    }
     c->out_cell = c->mem.alloc<uint16_t*>(1, &rc);
     c->stop_cell = c->mem.alloc<float*>(1, &rc);
     if (rc) return rc;
@@ -976,7 +1045,8 @@ int ming_cuda_finalize(ming_ctx* c) {
     CK(cudaMemcpy(c->bt, c->bt_host.data(), c->bt_host.size() * 4, cudaMemcpyHostToDevice));
     for (int p = f.max_pages - 1; p >= 0; p--) c->free_pages.push_back(p);
     c->seqs.assign(f.max_seqs, SeqInfo{});
-    if (f.layers > 0 && (rc = setup_mega(c))) return rc;
+    // the persistent kernel's attention sees every position
+    if (f.layers > 0 && !c->bounded && (rc = setup_mega(c))) return rc;
 
     // ---- flow head ----
     if (f.dit_mode != MING_DIT_NONE) {
@@ -1110,6 +1180,7 @@ int ming_cuda_seq_alloc(ming_ctx* c, int* id) {
             c->seqs[i] = SeqInfo{true, 0};
             const int zero = 0;
             CK(cudaMemcpyAsync(c->seq_len + i, &zero, 4, cudaMemcpyHostToDevice, c->stream));
+            if (c->seq_shift) CK(cudaMemcpyAsync(c->seq_shift + i, &zero, 4, cudaMemcpyHostToDevice, c->stream));
             *id = i;
             return MING_OK;
         }
@@ -1140,7 +1211,64 @@ int ming_cuda_seq_truncate(ming_ctx* c, int id, int len) {
     if (len < 0 || len > c->seqs[id].len) return fail(MING_ERR_INVALID, "truncate length out of range");
     c->seqs[id].len = len;
     CK(cudaMemcpyAsync(c->seq_len + id, &c->seqs[id].len, 4, cudaMemcpyHostToDevice, c->stream));
+    if (len == 0 && c->seq_shift) {
+        c->seqs[id].shift = 0;
+        CK(cudaMemcpyAsync(c->seq_shift + id, &c->seqs[id].shift, 4, cudaMemcpyHostToDevice, c->stream));
+    }
     CK(cudaStreamSynchronize(c->stream));
+    return MING_OK;
+}
+
+int ming_cuda_seq_evict(ming_ctx* c, int id, int keep, int sinks, int recent) {
+    if (!c || !c->finalized) return fail(MING_ERR_INVALID, "context not finalized");
+    int rc = check_seq(c, id);
+    if (rc) return rc;
+    const ming_cfg& f = c->cfg;
+    if (!c->bounded) return fail(MING_ERR_INVALID, "eviction needs a context with attn_window or kv_track");
+    if (sinks < 0 || recent < 0 || keep < 1 || (int64_t)sinks + recent > keep)
+        return fail(MING_ERR_INVALID, "sinks and recent must not be negative and fit in keep, which is at least 1");
+    if (!c->kv_acc && sinks + recent != keep) return fail(MING_ERR_INVALID, "without kv_track keep must be sinks + recent");
+    if (keep > AT_MAX_KEEP && sinks + recent != keep)
+        return fail(MING_ERR_INVALID, "keep is at most " + std::to_string(AT_MAX_KEEP) + " with totals");
+    SeqInfo& s = c->seqs[id];
+    if (s.len <= keep || f.layers < 1) return MING_OK;
+    CK(cudaSetDevice(c->device));
+    EvictOp e{};
+    e.from.ps = (int64_t)f.layers * 2 * f.kv_heads * PAGE * HD;
+    e.from.hs = PAGE * HD;
+    e.from.ss = HD;
+    e.from.k = c->pool;
+    e.from.v = c->pool + (int64_t)f.kv_heads * PAGE * HD;
+    e.from.bt = c->bt + (size_t)id * c->bt_ld;
+    e.from.lens = c->seq_len + id;
+    e.from.bt_ld = c->bt_ld;
+    e.from.pages = f.max_pages;
+    e.from.max_len = f.max_ctx;
+    e.to = e.from;
+    e.from_ls = e.to_ls = (int64_t)2 * f.kv_heads * PAGE * HD;
+    if (c->kv_acc) e.acc = e.acc_to = c->kv_acc + (int64_t)id * f.layers * f.kv_heads * f.max_ctx;
+    e.a_ls = e.t_ls = (int64_t)f.kv_heads * f.max_ctx;
+    e.a_hs = e.t_hs = f.max_ctx;
+    e.seqs = 1;
+    e.layers = f.layers;
+    e.kv_heads = f.kv_heads;
+    e.keep = keep;
+    e.sinks = sinks;
+    e.recent = recent;
+    e.err = c->dev_err;
+    CK(launch_kv_evict(e, c->stream));
+    s.shift += s.len - keep;
+    s.len = keep;
+    CK(cudaMemcpyAsync(c->seq_len + id, &s.len, 4, cudaMemcpyHostToDevice, c->stream));
+    CK(cudaMemcpyAsync(c->seq_shift + id, &s.shift, 4, cudaMemcpyHostToDevice, c->stream));
+    // pages behind the last position, queued behind the move
+    const int p0 = (keep + PAGE - 1) / PAGE;
+    for (int p = p0; p < c->bt_ld; p++) {
+        int& pg = c->bt_host[(size_t)id * c->bt_ld + p];
+        if (pg >= 0) c->free_pages.push_back(pg);
+        pg = -1;
+    }
+    if (p0 < c->bt_ld) CK(cudaMemsetAsync(c->bt + (size_t)id * c->bt_ld + p0, 0xff, (size_t)(c->bt_ld - p0) * 4, c->stream));
     return MING_OK;
 }
 
@@ -1160,6 +1288,11 @@ int ming_cuda_lm_prefill(ming_ctx* c, int s, const uint16_t* x, int L, uint16_t*
         for (int r = 0; r < n; r++) posv[r] = start + c0 + r;
         CK(cudaMemcpyAsync(c->row_seq, seqv.data(), n * 4, cudaMemcpyHostToDevice, c->stream));
         CK(cudaMemcpyAsync(c->row_pos, posv.data(), n * 4, cudaMemcpyHostToDevice, c->stream));
+        if (c->bounded) {
+            c->pf_seq = s;
+            const int meta[3] = {0, n, start + c0 + n};
+            CK(cudaMemcpyAsync(c->pf_meta, meta, sizeof(meta), cudaMemcpyHostToDevice, c->stream));
+        }
         if ((rc = copy_in(c, c->x, x + (size_t)c0 * H, (size_t)n * H * 2, kind))) return rc;
         const cudaError_t le = enqueue_layers(c, n, false);
         if (le != cudaSuccess) return fail(MING_ERR_CUDA, std::string("prefill attention launch: ") + cudaGetErrorString(le));
@@ -1360,7 +1493,7 @@ int ming_cuda_step_kernels(ming_ctx* c, int B, int* n) {
     int lin = 2;  // staged: prologue kernel + linear
     if (B <= 64 && c->lin.err && bulk_enabled()) lin = 1;
     else if (B <= 8) lin = 1;
-    const int attn = c->nsplit <= 8 ? 1 : 2;
+    const int attn = c->bounded || c->nsplit <= 8 ? 1 : 2;
     *n = 1 + (4 * lin + attn) * c->cfg.layers + 1;
     return MING_OK;
 }
@@ -1422,6 +1555,9 @@ int ming_cuda_kv_write(ming_ctx* c, int s, int layer, int pos0, int n, const uin
                                                             n, d, d + bytes / 2);
         e = cudaGetLastError();
     }
+    if (e == cudaSuccess && c->kv_acc)
+        e = cudaMemset2DAsync(c->kv_acc + ((size_t)s * c->cfg.layers + layer) * KH * c->cfg.max_ctx + pos0, (size_t)c->cfg.max_ctx * 4,
+                              0, (size_t)n * 4, KH, c->stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(c->stream);
     cudaFree(d);
     if (e != cudaSuccess) return fail(MING_ERR_CUDA, std::string("kv_write: ") + cudaGetErrorString(e));
@@ -1430,6 +1566,21 @@ int ming_cuda_kv_write(ming_ctx* c, int s, int layer, int pos0, int n, const uin
         CK(cudaMemcpyAsync(c->seq_len + s, &c->seqs[s].len, 4, cudaMemcpyHostToDevice, c->stream));
         CK(cudaStreamSynchronize(c->stream));
     }
+    return MING_OK;
+}
+
+int ming_cuda_kv_totals(ming_ctx* c, int s, int layer, int pos0, int n, float* out) {
+    if (!c || !c->finalized || !out) return fail(MING_ERR_INVALID, "bad argument");
+    if (!c->kv_acc) return fail(MING_ERR_INVALID, "the context does not track attention (kv_track)");
+    int rc = check_seq(c, s);
+    if (rc) return rc;
+    if (layer < 0 || layer >= c->cfg.layers || pos0 < 0 || n < 0 || pos0 > c->seqs[s].len - n)
+        return fail(MING_ERR_INVALID, "range out of bounds");
+    if (n == 0) return MING_OK;
+    CK(cudaStreamSynchronize(c->stream));
+    const size_t ld = c->cfg.max_ctx, KH = c->cfg.kv_heads;
+    CK(cudaMemcpy2D(out, (size_t)n * 4, c->kv_acc + ((size_t)s * c->cfg.layers + layer) * KH * ld + pos0, ld * 4, (size_t)n * 4, KH,
+                    cudaMemcpyDeviceToHost));
     return MING_OK;
 }
 
@@ -1540,6 +1691,7 @@ extern "C" int ming_cuda_lm_decode_noalloc(ming_ctx* c, int B, const int* ids, c
                                            float* stop, int kind) {
     if (!c || !c->finalized) return fail(MING_ERR_INVALID, "context not finalized");
     if (c->cfg.layers < 1) return fail(MING_ERR_INVALID, "no LM configured");
+    if (c->bounded) return fail(MING_ERR_INVALID, "allocation-free decode attends to every position: not with attn_window or kv_track");
     if (!ids || !x) return fail(MING_ERR_INVALID, "null argument");
     if (B < 1 || B > c->cfg.max_batch) return fail(MING_ERR_INVALID, "batch size out of range");
     const ming_cfg& f = c->cfg;

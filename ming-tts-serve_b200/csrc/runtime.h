@@ -75,6 +75,7 @@ struct DitBlockW {
 struct SeqInfo {
     bool live = false;
     int len = 0;
+    int shift = 0;  // positions evicted: the position after the cache's last is len + shift
 };
 
 }  // namespace rt
@@ -109,6 +110,13 @@ struct ming_ctx {
     std::vector<int> bt_host;
     std::vector<int> free_pages;
     std::vector<ming::rt::SeqInfo> seqs;
+    // attention over bounded caches (cfg.attn_window or cfg.kv_track)
+    bool bounded = false;
+    float* kv_acc = nullptr;   // kv_track: [max_seqs][layers][kv_heads][max_ctx] attention totals
+    float* lse = nullptr;      // kv_track: [maxr][heads] of a prefill chunk
+    int* seq_shift = nullptr;  // [max_seqs]
+    int* pf_meta = nullptr;    // a prefill chunk's q_start [2] and length
+    int pf_seq = 0;            // its sequence
 
     // activations / step state
     int maxr = 0, nsplit = 0;

@@ -37,6 +37,7 @@ SYMBOLS = [
     "ming_cuda_loop_step", "ming_cuda_loop_result", "ming_cuda_loop_destroy", "ming_cuda_load_safetensors",
     "ming_cuda_vae_decode",
     "ming_cuda_attn_prefill", "ming_cuda_attn_weights", "ming_cuda_attn_decode", "ming_cuda_kv_evict",
+    "ming_cuda_seq_evict", "ming_cuda_kv_totals",
 ]
 
 
@@ -47,7 +48,7 @@ class Cfg(ctypes.Structure):
             "weight_bits", "group_size", "page_size", "max_seqs", "max_pages", "max_ctx", "max_batch", "max_prefill",
             "dit_mode", "dit_hidden", "dit_blocks", "dit_heads", "dit_ff", "dit_latent", "dit_frames",
             "dit_cond_dim", "dit_freq_dim", "dit_max_batch", "agg_blocks", "vae_layers", "vae_ff", "vae_window",
-            "vae_max_latents")]
+            "vae_max_latents", "attn_window", "attn_sinks", "kv_track")]
 
 
 class SampleParams(ctypes.Structure):
@@ -135,6 +136,8 @@ def lib():
         "ming_cuda_loop_destroy": (I, [P]),
         "ming_cuda_load_safetensors": (I, [P, ctypes.c_char_p, IP]),
         "ming_cuda_vae_decode": (I, [P, P, I, P, I]),
+        "ming_cuda_seq_evict": (I, [P, I, I, I, I]),
+        "ming_cuda_kv_totals": (I, [P, I, I, I, I, P]),
         "ming_cuda_attn_prefill": (I, [P, P, P]),
         "ming_cuda_attn_weights": (I, [P, P, P]),
         "ming_cuda_attn_decode": (I, [P, P, P]),
@@ -331,6 +334,12 @@ class Context:
     def seq_truncate(self, s, n):
         _check(lib().ming_cuda_seq_truncate(self._h, s, n))
 
+    def seq_evict(self, s, keep, sinks=0, recent=0):
+        """Brings sequence s of a context with attn_window or kv_track back to
+        `keep` cached positions (the first `sinks`, the last `recent`, and the
+        most attended between); nothing if it holds no more."""
+        _check(lib().ming_cuda_seq_evict(self._h, s, keep, sinks, recent))
+
     def prefill(self, s, x, want_out=True):
         """x: uint16 [L, hidden] host array -> (out [L, hidden] uint16, stop [L] f32)."""
         x = np.ascontiguousarray(x, dtype=np.uint16)
@@ -407,6 +416,12 @@ class Context:
         v = np.empty((kh, n, 64), dtype=np.uint16)
         _check(lib().ming_cuda_kv_read(self._h, s, layer, pos0, n, _ptr(k), _ptr(v)))
         return k, v
+
+    def kv_totals(self, s, layer, pos0, n):
+        """Attention totals f32 [kv_heads, n] of positions pos0.. (kv_track)."""
+        out = np.empty((self.cfg.kv_heads, n), dtype=np.float32)
+        _check(lib().ming_cuda_kv_totals(self._h, s, layer, pos0, n, _ptr(out)))
+        return out
 
     def _latent_width(self):
         return self.cfg.dit_frames * self.cfg.dit_latent

@@ -119,6 +119,22 @@ def test_evict_arguments(to, bad, word):
     refused(M.lib().ming_cuda_kv_evict(None, ctypes.byref(cache()), ctypes.byref(cache(**to)), ctypes.byref(evict(**bad))), word)
 
 
+@pytest.mark.parametrize("bad", [dict(attn_window=-1), dict(attn_sinks=-1), dict(attn_sinks=4), dict(kv_track=2), dict(kv_track=-1)])
+def test_create_rejects_bad_bounds(bad):
+    _ensure_built()
+    c = M.default_cfg(**bad)
+    assert (M.default_cfg().attn_window, M.default_cfg().attn_sinks, M.default_cfg().kv_track) == (0, 0, 0)
+    h = ctypes.c_void_p()
+    refused(M.lib().ming_cuda_create(0, ctypes.byref(c), ctypes.byref(h)), "attn_" if "kv_track" not in bad else "kv_track")
+
+
+def test_sequence_calls_reject_a_null_context():
+    _ensure_built()
+    f = (ctypes.c_float * 4)()
+    refused(M.lib().ming_cuda_seq_evict(None, 0, 8, 0, 8), "finalized")
+    refused(M.lib().ming_cuda_kv_totals(None, 0, 0, 0, 1, f), "bad argument")
+
+
 def test_python_checks():
     torch = pytest.importorskip("torch")
     k = torch.zeros(4, 1, 2, 16, 64, dtype=torch.bfloat16)
