@@ -227,16 +227,19 @@ def _types():
 def _tensor(t, name, dtype, ndim, device):
     """Checks a device tensor; returns its strides, 0 for dimensions of one
     element, which are never strided over."""
-    if not hasattr(t, "get_device"):
-        raise MingError(f"{name}: a device tensor is wanted")
-    if t.dtype is not dtype or t.dim() != ndim:
-        raise MingError(f"{name}: {dtype} of {ndim} dimensions is wanted, got {t.dtype} of {t.dim()}")
-    if t.get_device() != device or device < 0:
-        raise MingError(f"{name}: a tensor on cuda:{max(device, 0)} is wanted, it is on {t.device}")
-    s, n = t.stride(), t.shape
-    if s[-1] != 1 and n[-1] > 1:
-        raise MingError(f"{name}: the last dimension must be contiguous")
-    return [0 if k == 1 else x for k, x in zip(n, s)] if 1 in n else s
+    try:
+        if t.dtype is dtype and t.ndim == ndim and t.get_device() == device >= 0:
+            s, n = t.stride(), t.shape
+            if 1 not in n:
+                if s[-1] == 1:
+                    return s
+            elif s[-1] == 1 or n[-1] == 1:
+                return [0 if k == 1 else x for k, x in zip(n, s)]
+            raise MingError(f"{name}: the last dimension must be contiguous")
+        raise MingError(f"{name}: {dtype} of {ndim} dimensions on cuda:{max(device, 0)} is wanted, got {t.dtype} of {t.ndim} "
+                        f"on {t.device}")
+    except AttributeError:
+        raise MingError(f"{name}: a device tensor is wanted") from None
 
 
 class KvCache:
@@ -269,8 +272,8 @@ class KvCache:
         if acc is None:
             return 0, 0, 0, 0
         s = _tensor(acc, name, _types()[1], 4, self.device)
-        n = acc.shape
-        if n[:3] != self.shape or n[3] < self.max_len:
+        *dims, n = acc.shape
+        if tuple(dims) != self.shape or n < self.max_len:
             raise MingError(f"{name}: [seqs, layers, kv_heads, at least max_len] is wanted")
         return acc.data_ptr(), s[0], s[1], s[2]
 
@@ -465,37 +468,44 @@ class Context:
         _check(lib().ming_cuda_kv_write(self._h, s, layer, pos0, k.shape[1], _ptr(k), _ptr(v)))
 
     def _attn(self, call, q, cache, out, q_start, max_rows, lse, acc, layer, window, sinks, scale, stream):
-        bf16, f32, i32 = _types()
-        if cache.device != self.device:
+        # every call runs this: one look at each attribute
+        device = self.device
+        if cache.device != device:
             raise MingError("the cache is on another device")
-        qs = _tensor(q, "q", bf16, 3, self.device)
+        bf16, f32, i32 = _types()
+        r, h, _ = _tensor(q, "q", bf16, 3, device)
         n = q.shape
-        if n[2] != 64:
+        rows, heads, dims = n
+        if dims != 64:
             raise MingError("q: heads of 64 dims are wanted")
-        o, os = 0, (0, 0)
+        o = o_r = o_h = start = z = a = a_s = a_l = a_h = 0
         if out is not None:
-            os = _tensor(out, "out", bf16, 3, self.device)
             if out.shape != n:
                 raise MingError("out and q differ in shape")
+            o_r, o_h, _ = _tensor(out, "out", bf16, 3, device)
             o = out.data_ptr()
-        start = z = 0
         if q_start is None:
-            if n[0] != cache.seqs:
+            if rows != cache.seqs:
                 raise MingError("q: one row per sequence is wanted")
         else:
-            _tensor(q_start, "q_start", i32, 1, self.device)
+            _tensor(q_start, "q_start", i32, 1, device)
             if q_start.shape[0] != cache.seqs + 1:
                 raise MingError("q_start: seqs + 1 entries are wanted")
             start = q_start.data_ptr()
+            if max_rows is None:
+                max_rows = rows
         if lse is not None:
-            _tensor(lse, "lse", f32, 2, self.device)
+            _tensor(lse, "lse", f32, 2, device)
             if lse.shape != n[:2] or not lse.is_contiguous():
                 raise MingError("lse: contiguous [rows, heads] is wanted")
             z = lse.data_ptr()
-        _ATTN.pack_into(self._args, 0, layer, n[1], window, sinks, scale or 0.0, q.data_ptr(), qs[0], qs[1], o, os[0], os[1],
-                        start, n[0], n[0] if max_rows is None else max_rows, z, *cache._acc(acc),
-                        0 if stream is None else stream or 1)
-        _check(call(self._h, cache.ref, self._args_at))
+        if acc is not None:
+            a, a_s, a_l, a_h = cache._acc(acc)
+        _ATTN.pack_into(self._args, 0, layer, heads, window, sinks, scale or 0.0, q.data_ptr(), r, h, o, o_r, o_h, start, rows,
+                        max_rows or 0, z, a, a_s, a_l, a_h, 0 if stream is None else stream or 1)
+        rc = call(self._h, cache.ref, self._args_at)
+        if rc:
+            _check(rc)
 
     def attn_prefill(self, q, q_start, cache, out, lse=None, *, max_rows=None, layer=0, window=0, sinks=0, scale=None,
                      stream=None):
@@ -505,7 +515,7 @@ class Context:
         most. stream: a CUDA stream's handle (0: the legacy default stream,
         None: the context's stream). Device tensors, asynchronous."""
         _want(q_start is not None and out is not None, "q_start and out are wanted")
-        self._attn(lib().ming_cuda_attn_prefill, q, cache, out, q_start, max_rows, lse, None, layer, window, sinks, scale, stream)
+        self._attn(_lib.ming_cuda_attn_prefill, q, cache, out, q_start, max_rows, lse, None, layer, window, sinks, scale, stream)
         return out
 
     def attn_weights(self, q, q_start, cache, lse, acc, *, max_rows=None, layer=0, window=0, sinks=0, scale=None,
@@ -513,13 +523,13 @@ class Context:
         """ming_cuda_attn_weights: the weights of attn_prefill's rows (its lse)
         added to acc f32 [seqs, layers, kv_heads, >= max_len]."""
         _want(q_start is not None, "q_start is wanted")
-        self._attn(lib().ming_cuda_attn_weights, q, cache, None, q_start, max_rows, lse, acc, layer, window, sinks, scale, stream)
+        self._attn(_lib.ming_cuda_attn_weights, q, cache, None, q_start, max_rows, lse, acc, layer, window, sinks, scale, stream)
         return acc
 
     def attn_decode(self, q, cache, out, acc=None, *, layer=0, window=0, sinks=0, scale=None, stream=None):
         """ming_cuda_attn_decode: one new token per sequence, q and out bf16
         [seqs, heads, 64]; its weights are added to acc unless that is None."""
-        self._attn(lib().ming_cuda_attn_decode, q, cache, out, None, None, None, acc, layer, window, sinks, scale, stream)
+        self._attn(_lib.ming_cuda_attn_decode, q, cache, out, None, None, None, acc, layer, window, sinks, scale, stream)
         return out
 
     def kv_evict(self, cache, to=None, acc=None, acc_to=None, *, keep, sinks=0, recent=0, index=None, stream=None):
