@@ -68,25 +68,38 @@ __global__ void __launch_bounds__(WT_THREADS, WT_PER_SM)
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(at_su32(slot)), "r"(AT_N) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
-    if (tid == 0) {
-        at_bar_init(k_full, 1);
-        for (int i = 0; i < WT_STAGES; i++) {
-            at_bar_init(&q_full[i], 2);
-            at_bar_init(&q_empty[i], 5);
+    // The copying warp sets the barriers up and starts its first copies without
+    // waiting for the others.
+    auto copy_q = [&](int s) {
+        const int st = s % WT_STAGES;
+        at_expect(&q_full[st], (uint32_t)(per * G * 128));
+        at_copy_q(sq + st * AT_TILE, &mq, kh * G, r0 + lo + (t0 + s) * per, &q_full[st]);
+    };
+    if (warp == 5) {
+        int page = a.kv.pages;
+        if (lane < AT_BLOCK_PAGES && j0 / AT_PAGE + lane < (len + AT_PAGE - 1) / AT_PAGE)
+            page = at_page(a.kv, a.kv.bt + (size_t)seq * a.kv.bt_ld, j0 / AT_PAGE + lane, a.err);
+        if (lane == 0) {
+            at_bar_init(k_full, 1);
+            for (int i = 0; i < WT_STAGES; i++) {
+                at_bar_init(&q_full[i], 2);
+                at_bar_init(&q_empty[i], 5);
+            }
+            at_bar_init(s_full, 1);
+            at_bar_init(s_read, 4);
+            asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+            at_async_fence();
+            for (int s = 0; s < min(steps, WT_STAGES); s++) copy_q(s);
+            if (steps > 0) at_expect(k_full, AT_TILE);
         }
-        at_bar_init(s_full, 1);
-        at_bar_init(s_read, 4);
-        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        __syncwarp();
+        if (steps > 0 && lane < AT_BLOCK_PAGES) at_copy_page(sk + lane * (AT_PAGE * 128), &mk, kh, page, k_full);
+    } else {
+        // columns that the copies never reach
+        const int tail = (AT_M - per * G) * 8;
+        for (int e = tid; e < WT_STAGES * tail; e += WT_THREADS - 32)
+            *reinterpret_cast<uint4*>(sq + e / tail * AT_TILE + (per * G + e % tail / 8) * 128 + (e % 8) * 16) = make_uint4(0, 0, 0, 0);
     }
-    // columns that the copies never reach
-    for (int e = tid; e < WT_STAGES * (AT_M - per * G) * 8; e += WT_THREADS) {
-        const int st = e / ((AT_M - per * G) * 8), k = e % ((AT_M - per * G) * 8);
-        *reinterpret_cast<uint4*>(sq + st * AT_TILE + (per * G + k / 8) * 128 + (k % 8) * 16) = make_uint4(0, 0, 0, 0);
-    }
-    // the tile's pages, looked up before they are needed
-    int page = a.kv.pages;
-    if (warp == 5 && lane < AT_BLOCK_PAGES && j0 / AT_PAGE + lane < (len + AT_PAGE - 1) / AT_PAGE)
-        page = at_page(a.kv, a.kv.bt + (size_t)seq * a.kv.bt_ld, j0 / AT_PAGE + lane, a.err);
     at_async_fence();
     at_before();
     __syncthreads();
@@ -116,27 +129,21 @@ __global__ void __launch_bounds__(WT_THREADS, WT_PER_SM)
             __syncwarp();
         }
     } else if (warp == 5) {
-        if (steps > 0) {
-            if (lane == 0) at_expect(k_full, AT_TILE);
-            __syncwarp();
-            if (lane < AT_BLOCK_PAGES) at_copy_page(sk + lane * (AT_PAGE * 128), &mk, kh, page, k_full);
-        }
+        // a column's row and head, the same in every tile
+        int off[AT_M / 32];
+#pragma unroll
+        for (int k = 0; k < AT_M / 32; k++) off[k] = (k * 32 + lane) / G * a.heads + kh * G + (k * 32 + lane) % G;
 #pragma unroll 1
         for (int s = 0; s < steps; s++) {
             const int st = s % WT_STAGES, i0 = lo + (t0 + s) * per, m = min(per, rows - i0) * G;  // columns that are rows
-            float z[AT_M / 32];
-#pragma unroll
-            for (int k = 0; k < AT_M / 32; k++) {
-                const int c = k * 32 + lane;
-                z[k] = c < m ? -AT_LOG2E * a.lse[(size_t)(r0 + i0 + c / G) * a.heads + kh * G + c % G] : -INFINITY;
+            if (s >= WT_STAGES) {
+                if (!(ok = at_wait_warp(&q_empty[st], ((s / WT_STAGES) - 1) & 1))) break;
+                if (lane == 0) copy_q(s);
             }
-            if (s >= WT_STAGES && !(ok = at_wait_warp(&q_empty[st], ((s / WT_STAGES) - 1) & 1))) break;
-            if (lane == 0) {
-                at_expect(&q_full[st], (uint32_t)(per * G * 128));
-                at_copy_q(sq + st * AT_TILE, &mq, kh * G, r0 + i0, &q_full[st]);
-            }
+            const float* from = a.lse + (size_t)(r0 + i0) * a.heads;
 #pragma unroll
-            for (int k = 0; k < AT_M / 32; k++) nlse[st * AT_M + k * 32 + lane] = z[k];
+            for (int k = 0; k < AT_M / 32; k++)
+                nlse[st * AT_M + k * 32 + lane] = k * 32 + lane < m ? -AT_LOG2E * from[off[k]] : -INFINITY;
             __syncwarp();
             if (lane == 0) at_arrive(&q_full[st]);
         }
