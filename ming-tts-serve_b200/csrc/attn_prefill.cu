@@ -161,29 +161,36 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
-    if (tid == 0) {
-        for (int i = 0; i < PF_STAGES; i++) {
-            at_bar_init(&landed[i], 1);
-            at_bar_init(&full[i], 1);
-            at_bar_init(&empty[i], 1);
-        }
-        for (int t = 0; t < 2; t++) {
-            at_bar_init(&q_full[t], 1);
-            at_bar_init(&q_empty[t], 1);
-            at_bar_init(&o_full[t], 1);
-        }
-        for (int i = 0; i < PF_BUFS; i++) {
-            at_bar_init(&s_full[i], 1);
-            at_bar_init(&p_ready[i], 4);
-        }
-        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-    }
     PfItems items(a, nx, total);  // the first one is on its way meanwhile
     PfItem it;
-    at_before();
-    __syncthreads();
-    at_after();
-    const uint32_t tmem = *slot;
+    // The copying warp sets the barriers up and goes ahead; the others meet.
+    if (warp == 9) {
+        if (lane == 0) {
+            for (int i = 0; i < PF_STAGES; i++) {
+                at_bar_init(&landed[i], 1);
+                at_bar_init(&full[i], 1);
+                at_bar_init(&empty[i], 1);
+            }
+            for (int t = 0; t < 2; t++) {
+                at_bar_init(&q_full[t], 1);
+                at_bar_init(&q_empty[t], 1);
+                at_bar_init(&o_full[t], 1);
+            }
+            for (int i = 0; i < PF_BUFS; i++) {
+                at_bar_init(&s_full[i], 1);
+                at_bar_init(&p_ready[i], 4);
+            }
+            asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+            at_async_fence();
+        }
+        __syncwarp();
+        asm volatile("barrier.cta.arrive 1, %0;\n" ::"n"(PF_THREADS) : "memory");
+    } else {
+        at_before();
+        asm volatile("barrier.cta.sync 1, %0;\n" ::"n"(PF_THREADS) : "memory");
+        at_after();
+    }
+    const uint32_t tmem = warp == 9 ? 0 : *slot;
     bool ok = true;
     if (warp == 8) {
         // The whole warp runs this role and one elected lane issues: the
