@@ -31,29 +31,30 @@ MING_DEV int ev_scan(int x, int lane) {  // inclusive
 }
 }  // namespace
 
-// A cluster per (sequence, layer, kv head). Which positions stay: the first
-// `sinks`, the last `recent`, and of those between the keep - sinks - recent
-// of the largest total. Its CTAs each find them for themselves (the totals are
-// a sixtieth of the rows' bytes and stay in the L1) and move a part of every
-// row each: K or V, and of it 128 / SPLIT bytes. Parts of a row do not meet, so
-// the move may be in place without a word between the CTAs; only the totals,
-// which all of them read, wait for the cluster before they are overwritten.
+// A CTA, or a cluster of PARTS, per (sequence, layer, kv head). Which positions
+// stay: the first `sinks`, the last `recent`, and of those between the keep -
+// sinks - recent of the largest total. A cluster's CTAs each find them for
+// themselves (the totals are a sixtieth of the rows' bytes and stay in the L1)
+// and move 128 / PARTS bytes of every row of K and V each. Parts of a row do
+// not meet, so the move may be in place without a word between the CTAs; only
+// the totals, which all of them read, wait for the cluster before they are
+// overwritten.
 //  * The smallest total that stays is found digit by digit: a histogram in
 //    shared memory, scanned from the top; the search ends early when a bin is
 //    taken whole. Positions that tie with it stay from the lowest on.
 //  * A warp counts its stretch of the positions, eight counts are summed, and
 //    the warp writes its kept positions to the list: two passes, one barrier.
-//  * Rows move EV_AHEAD x 256 x 16 bytes at a time, read before they are
+//  * Rows move EV_AHEAD to a thread at a time, K and V together, read before they are
 //    written. A row's place is never behind it, so what a batch writes no
 //    later one reads, and the next batch is read meanwhile.
 // Bound by the kept rows' bytes in a batch of sequences, by the chain of
 // dependent loads (length, totals, three histograms, pages, rows) for one.
-template <int SPLIT>
-__global__ void __launch_bounds__(EV_THREADS, 4) kv_evict_kernel(const EvictOp a) {
+template <int PARTS>
+__global__ void __launch_bounds__(EV_THREADS, 2) kv_evict_kernel(const EvictOp a) {
     extern __shared__ int ev_list[];  // positions that stay, ascending (when some between do and some do not)
     __shared__ int hist[EV_BINS], warp_sum[EV_WARPS], warp_ties[EV_WARPS];
     __shared__ int s_digit, s_left, s_bin;
-    constexpr int PARTS = 2 * SPLIT, LANES = 8 / SPLIT, ROWS = EV_THREADS / LANES;  // CTAs, lanes of a row, rows at once
+    constexpr int LANES = 8 / PARTS, ROWS = EV_THREADS / LANES;  // lanes of a row, rows at once
     const int part = blockIdx.x % PARTS, kh = blockIdx.x / PARTS, layer = blockIdx.y, b = blockIdx.z;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int seq = at_seq(a.from, b), n = at_len_of(a.from, seq, a.err), kept = min(a.keep, n);
@@ -137,56 +138,57 @@ __global__ void __launch_bounds__(EV_THREADS, 4) kv_evict_kernel(const EvictOp a
         __syncthreads();
     }
     // everyone has read the totals: they may be overwritten behind the matching wait
-    if (acc) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+    if (acc && PARTS > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
     // the position that moves to place s
     const int skipped = n - kept;
     auto source = [&](int s) { return s < lo ? s : s >= kept - (n - hi) || !some ? s + (s < lo + need ? 0 : skipped) : ev_list[s]; };
 
     const int* bt = a.from.bt + (size_t)seq * a.from.bt_ld;
     const int* bt_to = a.to.bt + (size_t)seq * a.to.bt_ld;
-    const bool values = part >= SPLIT;
-    const uint16_t* src = (values ? a.from.v : a.from.k) + layer * a.from_ls + kh * a.from.hs;
-    uint16_t* dst = (values ? a.to.v : a.to.k) + layer * a.to_ls + kh * a.to.hs;
-    const int col = (part % SPLIT) * (AT_HD / SPLIT) + (tid % LANES) * 8, row = tid / LANES;
-    const bool in_place = src == dst && bt == bt_to;
-    auto read = [&](int s0, uint4 (&v)[EV_AHEAD]) {
+    const int col = part * (AT_HD / PARTS) + (tid % LANES) * 8, row = tid / LANES;
+    const int64_t from0 = layer * a.from_ls + kh * a.from.hs + col, to0 = layer * a.to_ls + kh * a.to.hs + col;
+    const bool in_place = a.from.k == a.to.k && a.from.v == a.to.v && bt == bt_to;
+    auto read = [&](int s0, uint4 (&v)[EV_AHEAD][2]) {
 #pragma unroll
         for (int i = 0; i < EV_AHEAD; i++) {
             const int s = s0 + i * ROWS + row;
             if (s >= kept) continue;
             const int p = source(s);
-            v[i] = *reinterpret_cast<const uint4*>(src + (int64_t)at_page(a.from, bt, p / AT_PAGE, a.err) * a.from.ps +
-                                                   (p % AT_PAGE) * a.from.ss + col);
+            const int64_t at = from0 + (int64_t)at_page(a.from, bt, p / AT_PAGE, a.err) * a.from.ps + (p % AT_PAGE) * a.from.ss;
+            v[i][0] = *reinterpret_cast<const uint4*>(a.from.k + at);
+            v[i][1] = *reinterpret_cast<const uint4*>(a.from.v + at);
         }
     };
-    uint4 v[EV_AHEAD], w[EV_AHEAD];
+    uint4 v[EV_AHEAD][2], w[EV_AHEAD][2];
     // in place, the first places often are the positions themselves
     int s0 = in_place ? lo / (EV_AHEAD * ROWS) * (EV_AHEAD * ROWS) : 0;
     if (in_place && skipped == 0) s0 = kept;
     if (s0 < kept) read(s0, v);
     for (; s0 < kept; s0 += EV_AHEAD * ROWS) {
         __syncthreads();  // the batch is read
-        const bool more = s0 + EV_AHEAD * ROWS < kept;
-        if (more) read(s0 + EV_AHEAD * ROWS, w);
+        if (s0 + EV_AHEAD * ROWS < kept) read(s0 + EV_AHEAD * ROWS, w);
 #pragma unroll
         for (int i = 0; i < EV_AHEAD; i++) {
             const int s = s0 + i * ROWS + row;
             if (s >= kept) continue;
             const int page = bt_to[s / AT_PAGE];
-            if ((unsigned)page < (unsigned)a.to.pages)
-                *reinterpret_cast<uint4*>(dst + (int64_t)page * a.to.ps + (s % AT_PAGE) * a.to.ss + col) = v[i];
-            else
+            if ((unsigned)page < (unsigned)a.to.pages) {
+                const int64_t at = to0 + (int64_t)page * a.to.ps + (s % AT_PAGE) * a.to.ss;
+                *reinterpret_cast<uint4*>(a.to.k + at) = v[i][0];
+                *reinterpret_cast<uint4*>(a.to.v + at) = v[i][1];
+            } else {
                 at_flag(a.err, AT_ERR_PAGE);
+            }
         }
 #pragma unroll
-        for (int i = 0; i < EV_AHEAD; i++) v[i] = w[i];
+        for (int i = 0; i < EV_AHEAD; i++) v[i][0] = w[i][0], v[i][1] = w[i][1];
     }
     if (part == 0 && a.index) {
         int* index = a.index + (((size_t)b * a.layers + layer) * a.kv_heads + kh) * a.keep;
         for (int s = tid; s < a.keep; s += EV_THREADS) index[s] = s < kept ? source(s) : -1;
     }
     __syncwarp();
-    if (acc) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    if (acc && PARTS > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
     if (acc && part == PARTS - 1) {
         float* acc_to = a.acc_to + seq * a.t_ss + layer * a.t_ls + kh * a.t_hs;
         for (int s = tid; s < (kept + EV_THREADS - 1) / EV_THREADS * EV_THREADS; s += EV_THREADS) {
@@ -203,25 +205,29 @@ cudaError_t launch_kv_evict(const EvictOp& a, cudaStream_t s) {
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {
-        const void* f[2] = {(const void*)kv_evict_kernel<1>, (const void*)kv_evict_kernel<2>};
+        const void* f[3] = {(const void*)kv_evict_kernel<1>, (const void*)kv_evict_kernel<2>, (const void*)kv_evict_kernel<4>};
         for (const void* k : f)
             if ((e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, AT_MAX_KEEP * 4)) != cudaSuccess) return e;
         if (dev < 64) ready[dev].store(true, std::memory_order_release);
     }
-    const bool four = (long long)a.seqs * a.layers * a.kv_heads * 2 < 2 * 148;  // few heads: four CTAs each, half rows
+    // few heads: several CTAs each
+    const long long heads = (long long)a.seqs * a.layers * a.kv_heads;
+    const int parts = heads * 2 <= 148 ? 4 : heads <= 2 * 148 ? 2 : 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.kv_heads * (four ? 4 : 2), a.layers, a.seqs);
+    cfg.gridDim = dim3(a.kv_heads * parts, a.layers, a.seqs);
     cfg.blockDim = dim3(EV_THREADS);
     cfg.dynamicSmemBytes = a.sinks + a.recent < a.keep ? (size_t)a.keep * 4 : 0;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = four ? 4 : 2;
+    at[0].val.clusterDim.x = parts;
     at[0].val.clusterDim.y = 1;
     at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return four ? cudaLaunchKernelEx(&cfg, kv_evict_kernel<2>, a) : cudaLaunchKernelEx(&cfg, kv_evict_kernel<1>, a);
+    return parts == 4   ? cudaLaunchKernelEx(&cfg, kv_evict_kernel<4>, a)
+           : parts == 2 ? cudaLaunchKernelEx(&cfg, kv_evict_kernel<2>, a)
+                        : cudaLaunchKernelEx(&cfg, kv_evict_kernel<1>, a);
 }
 
 }  // namespace ming
