@@ -290,7 +290,10 @@ typedef struct ming_kv_cache {
  * multiple of kv_heads with at most 8 query heads per kv head. Row r, head h
  * of q is at q + r * q_row_stride + h * q_head_stride (16-byte aligned,
  * strides multiples of 8). A row that sees nothing gets zeros and a
- * log-sum-exp of -infinity. */
+ * log-sum-exp of -infinity. Keys and values at positions that no row of the
+ * call sees may hold anything. At positions that some rows see and others do
+ * not (a prompt's diagonal, the edges of its window) an infinite or NaN value
+ * may reach the others' outputs; keys there reach only rows that see them. */
 typedef struct ming_attn {
     int layer, heads, window, sinks;
     float scale;

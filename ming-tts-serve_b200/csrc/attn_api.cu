@@ -88,6 +88,10 @@ int attn_op(ming_ctx* c, const ming_kv_cache* kv, const ming_attn* f, bool promp
     if (misaligned(f->lse, 4) || misaligned(f->acc, 4)) return fail(MING_ERR_INVALID, "lse and acc must be 4-byte aligned");
     if (f->acc && (f->acc_seq_stride < 0 || f->acc_layer_stride < 0 || f->acc_head_stride < 0))
         return fail(MING_ERR_INVALID, "acc: negative stride");
+    // the copies of a prompt's operands step over every dimension that has more than one element
+    if (prompt && ((kv->pages > 1 && !kv->page_stride) || (kv->kv_heads > 1 && !kv->head_stride) || (f->heads > 1 && !f->q_head_stride) ||
+                   (f->rows > 1 && !f->q_row_stride)))
+        return fail(MING_ERR_INVALID, "the strides of pages, heads and rows must not be 0");
     *a = AttnOp{};
     a->kv = pages_of(kv, f->layer);
     a->q = f->q;
@@ -107,8 +111,9 @@ int attn_op(ming_ctx* c, const ming_kv_cache* kv, const ming_attn* f, bool promp
     a->heads = f->heads;
     a->kv_heads = kv->kv_heads;
     a->group = f->heads / kv->kv_heads;
-    a->window = f->window;
-    a->sinks = f->sinks;
+    // a window as long as the cache hides nothing
+    a->window = f->window < kv->max_len ? f->window : 0;
+    a->sinks = f->sinks < kv->max_len ? f->sinks : kv->max_len;
     a->scale_log2 = (f->scale == 0.f ? 0.125f : f->scale) * AT_LOG2E;
     a->err = c ? c->dev_err : nullptr;
     return MING_OK;

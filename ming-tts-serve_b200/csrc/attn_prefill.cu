@@ -68,13 +68,8 @@ struct BlockSpan {
 struct PfItem {
     int kh, b, x;     // kv head, row of the batch, which rows
     int r0, r1, len;  // as read: rows of q, positions held
-    MING_DEV PfItem() {}
     // The loads alone: their checks wait until the item's turn.
-    MING_DEV void read(const AttnOp& a, int w, int nx) {
-        const int per = a.kv_heads * a.seqs, rest = w % per;
-        x = nx - 1 - w / per;
-        b = rest / a.kv_heads;
-        kh = rest % a.kv_heads;
+    MING_DEV void read(const AttnOp& a) {
         r0 = a.q_start[b];
         r1 = a.q_start[b + 1];
         len = a.kv.lens[at_seq(a.kv, b)];
@@ -84,18 +79,32 @@ struct PfItem {
         len = at_len(a.kv, len + a.kv.len_add, a.err);
     }
 };
-// A CTA's items in turn, each read while the one before it is worked on.
+// A CTA's items in turn, kv heads fastest, then sequences, then rows from the
+// last on; each is read while the one before it is worked on. The step from
+// one to the next is a division made once.
 struct PfItems {
     const AttnOp& a;
-    int w, nx, total;
+    int dkh, db, dx;
     PfItem ahead;
-    MING_DEV PfItems(const AttnOp& a_, int nx_, int total_) : a(a_), w(blockIdx.x), nx(nx_), total(total_) {
-        if (w < total) ahead.read(a, w, nx);
+    MING_DEV PfItems(const AttnOp& a_, int nx) : a(a_) {
+        const int g = gridDim.x, w = blockIdx.x;
+        dkh = g % a.kv_heads;
+        db = g / a.kv_heads % a.seqs;
+        dx = g / a.kv_heads / a.seqs;
+        ahead.kh = w % a.kv_heads;
+        ahead.b = w / a.kv_heads % a.seqs;
+        ahead.x = nx - 1 - w / a.kv_heads / a.seqs;
+        if (ahead.x >= 0) ahead.read(a);
     }
     MING_DEV bool next(PfItem& it) {
-        if (w >= total) return false;
+        if (ahead.x < 0) return false;
         it = ahead;
-        if ((w += gridDim.x) < total) ahead.read(a, w, nx);
+        ahead.kh += dkh;
+        ahead.b += db;
+        ahead.x -= dx;
+        if (ahead.kh >= a.kv_heads) ahead.kh -= a.kv_heads, ahead.b++;
+        if (ahead.b >= a.seqs) ahead.b -= a.seqs, ahead.x--;
+        if (ahead.x >= 0) ahead.read(a);
         it.check(a);
         return true;
     }
@@ -154,14 +163,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(&mv)) : "memory");
     }
     const int G = a.group, per = AT_M / G, step = tiles * per;  // positions of a tile, of an item
-    const int total = nx * a.kv_heads * a.seqs;
 
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(at_su32(slot)), "r"(PF_COLS)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
-    PfItems items(a, nx, total);  // the first one is on its way meanwhile
+    PfItems items(a, nx);  // the first one is on its way meanwhile
     PfItem it;
     // The copying warp sets the barriers up and goes ahead; the others meet.
     if (warp == 9) {

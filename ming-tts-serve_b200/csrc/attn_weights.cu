@@ -62,6 +62,10 @@ __global__ void __launch_bounds__(WT_THREADS, WT_PER_SM)
     const int j0 = tile * AT_N, lo = max(0, j0 - first), last = min(j0 + AT_N, len) - 1;
     const int hi = a.window && j0 >= a.sinks ? (int)min((long long)rows, (long long)last + a.window - first) : rows;
     if (j0 >= len || lo >= hi) return;  // the whole cluster
+    // This CTA runs: the others may write to its memory once all have said so.
+    // (Said before tensor memory is asked for, so that no one holds any while
+    // it waits for a CTA that cannot get some.)
+    if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
     const int nt = (hi - lo + per - 1) / per, t0 = (int)((long long)nt * rank / split), steps = (int)((long long)nt * (rank + 1) / split) - t0;
 
     if (warp == 4) {
@@ -104,8 +108,6 @@ __global__ void __launch_bounds__(WT_THREADS, WT_PER_SM)
     at_before();
     __syncthreads();
     at_after();
-    // (the others' memory is written to only when this has completed)
-    if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
     const uint32_t tmem = *slot;
     bool ok = true;
     float total = 0.f;

@@ -394,8 +394,8 @@ cudaError_t enqueue_bounded_attn(ming_ctx* c, int layer, int rows, bool decode) 
     a.heads = f.heads;
     a.kv_heads = f.kv_heads;
     a.group = f.heads / f.kv_heads;
-    a.window = f.attn_window;
-    a.sinks = f.attn_sinks;
+    a.window = f.attn_window < f.max_ctx ? f.attn_window : 0;
+    a.sinks = f.attn_sinks < f.max_ctx ? f.attn_sinks : f.max_ctx;
     a.scale_log2 = 0.125f * AT_LOG2E;
     a.a_ss = (int64_t)f.layers * f.kv_heads * f.max_ctx;
     a.a_hs = f.max_ctx;

@@ -95,6 +95,18 @@ def test_arguments_of_one_operator(op, bad, word):
     refused(call(op, cache(), attn(**{**OPS[op], **bad})), word)
 
 
+@pytest.mark.parametrize("op", ["prefill", "weights"])
+@pytest.mark.parametrize("c,a", [(dict(page_stride=0), {}), (dict(head_stride=0), {}), ({}, dict(q_head_stride=0)),
+                                 ({}, dict(q_row_stride=0))])
+def test_a_prompt_steps_over_its_strides(op, c, a):
+    refused(call(op, cache(**c), attn(**{**OPS[op], **a})), "must not be 0")
+    one = dict(pages=1) if "page_stride" in c else dict(kv_heads=1) if "head_stride" in c else {}
+    if one:  # nothing to step over
+        refused(call(op, cache(**c, **one), attn(**{**OPS[op], "heads": 7 * one.get("kv_heads", 2)})), "null context")
+    else:
+        refused(call("decode", cache(), attn(**a)), "null context")
+
+
 def test_null_structures():
     for op in OPS:
         refused(call(op, None, attn()), "null")

@@ -244,6 +244,51 @@ def test_prefill_sharp(ctx):
     check_prefill(ctx, Case([600], [600], 14, 2, 90, 4, sharp=60.0, seed=14))
 
 
+@pytest.mark.parametrize("window,sinks", [(2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1), (5, 2 ** 31 - 1), (700, 699), (699, 1)])
+def test_windows_and_sinks_of_any_size(ctx, window, sinks):
+    check_prefill(ctx, Case([700], [650], 14, 2, window, sinks, poison=False, seed=3))
+    check_decode(ctx, Case([700], [1], 14, 2, window, sinks, poison=False, seed=3))
+
+
+def test_keys_that_some_rows_do_not_see(ctx):
+    """A NaN key reaches the rows that see it and no others; the same with an infinite one."""
+    for bad in (math.nan, math.inf, -math.inf):
+        c = Case([300], [300], 14, 2, 100, 4, poison=False, seed=5)
+        clean, _ = run_prefill(ctx, c)
+        c.k[c.bt[0, 9].long(), 0, 1, 3] = bad  # position 147, kv head 1
+        out, lse = run_prefill(ctx, c)
+        hit = torch.zeros(300, 14, dtype=torch.bool, device="cuda")
+        hit[147:247, 7:] = True
+        assert torch.equal(out[~hit], clean[~hit])
+        assert out[hit].isnan().any(-1).all() if math.isnan(bad) else True
+        d = Case([300], [1], 14, 2, 100, 4, poison=False, seed=5)
+        want, got = torch.empty_like(d.q), torch.empty_like(d.q)
+        s = torch.cuda.current_stream().cuda_stream
+        ctx.attn_decode(d.q, d.cache, want, window=100, sinks=4, stream=s)
+        d.k[d.bt[0, 9].long(), 0, 1, 3] = bad
+        d.v[d.bt[0, 9].long(), 0, 1, 3] = bad
+        ctx.attn_decode(d.q, d.cache, got, window=100, sinks=4, stream=s)
+        assert torch.equal(want, got)
+
+
+def test_strided_totals(ctx):
+    """Totals in any strides: every second sequence of a larger buffer, heads outermost."""
+    c = Case([200, 333], [200, 40], 14, 2, 50, 3, layers=2, layer=1, seed=6)
+    base = torch.rand(2, 2, 5, 400, device="cuda")  # [kv head, layer, sequence, position]
+    view = base.permute(2, 1, 0, 3)[1:5:2]
+    view[..., :c.acc0.shape[-1]].copy_(c.acc0)
+    before = base.clone()
+    out, lse = run_prefill(ctx, c)
+    s = torch.cuda.current_stream().cuda_stream
+    ctx.attn_weights(c.q, c.q_start, c.cache, lse, view, max_rows=200, layer=1, window=50, sinks=3, stream=s)
+    acc = c.acc0.clone()
+    ctx.attn_weights(c.q, c.q_start, c.cache, lse, acc, max_rows=200, layer=1, window=50, sinks=3, stream=s)
+    torch.cuda.synchronize()
+    assert torch.equal(view[..., :acc.shape[-1]], acc)
+    changed = base != before
+    assert not changed[:, 0].any() and not changed[:, :, ::2].any() and not changed[..., acc.shape[-1]:].any()
+
+
 def test_prefill_more_rows_than_positions(ctx):
     """Rows at negative positions see nothing."""
     c = Case([5], [9], 14, 2)

@@ -245,6 +245,36 @@ def test_generate_and_written_caches(weights, plain):
     ctx.close()
 
 
+def test_sampling_loop_on_a_window(cuda_ok):
+    """The sampling loop runs on a bounded context: a window that hides nothing
+    gives the ordinary loop's first step (later ones feed on its rounding), a
+    short one runs its budget; two requests share a step."""
+    Wl = synth.lm_weights(seed=31, bits=4, layers=2, qscale=QS)
+    Wl["stop_head.bias"] = synth.f32_to_bf16(np.array([0.0, -4.0], np.float32))
+    Wf = synth.flow_weights(seed=32, blocks=2, hidden=512, ff=1024)
+    Wa = synth.agg_weights(seed=33, blocks=2, hidden=512, ff=1024)
+    kw = dict(layers=2, weight_bits=4, dit_mode=M.DIT_TOKEN, dit_hidden=512, dit_blocks=2, dit_heads=8, dit_ff=1024, agg_blocks=2,
+              dit_max_batch=8, max_ctx=512, max_pages=256, max_batch=8, max_seqs=8)
+    embeds = synth.normal_bf16(9, "loop.prompt", (40, H))
+    got = {}
+    for name, extra in (("plain", {}), ("wide", dict(attn_window=512, kv_track=1)), ("short", dict(attn_window=16, attn_sinks=2))):
+        ctx = M.Context(M.default_cfg(**kw, **extra), weights={**Wl, **Wf, **Wa})
+        p = M.sample_params(max_steps=8)
+        lat, zt, st = ctx.sample_latents(embeds, params=p, seed=3, trace=True)
+        assert lat.shape[0] == 8 and np.isfinite(bf(lat)).all()
+        got[name] = (bf(lat), bf(zt))
+        loop = M.Loop(ctx, 2, p)
+        ids = [loop.submit(embeds[:n], seed=3) for n in (40, 25)]
+        while loop.step()[0]:
+            pass
+        res = [loop.result(i) for i in ids]
+        assert all(r[0].shape[0] == 8 for r in res)
+        loop.close()
+        ctx.close()
+    cos = lambda a, b: (a * b).sum() / np.linalg.norm(a) / np.linalg.norm(b)  # noqa: E731
+    assert cos(got["plain"][1][0], got["wide"][1][0]) > 0.999 and cos(got["plain"][0][0], got["wide"][0][0]) > 0.999
+
+
 def test_refusals(weights, plain):
     pctx, _ = plain
     ps = pctx.seq_alloc()
