@@ -47,7 +47,8 @@ __global__ void __launch_bounds__(WT_THREADS, WT_PER_SM)
     uint32_t* slot = reinterpret_cast<uint32_t*>(s_read + 1);
     float* part = reinterpret_cast<float*>(slot + 4);  // an owner's: [rank][AT_N / owners], all ranks' sums of its positions
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-    const int rank = blockIdx.x % split, tile = blockIdx.x / split, kh = blockIdx.y, b = blockIdx.z;
+    // the first tiles of every sequence, which the most rows see, start first
+    const int rank = blockIdx.x % split, kh = blockIdx.x / split % a.kv_heads, b = blockIdx.x / split / a.kv_heads, tile = blockIdx.y;
     const int G = a.group, per = AT_M / G;
     const int seq = at_seq(a.kv, b);
     int r0 = a.q_start[b], r1 = a.q_start[b + 1];
@@ -237,10 +238,11 @@ cudaError_t launch_attn_weights(const AttnOp& a, cudaStream_t s) {
     if (!at_q_map(&mq, a, per) || !at_page_map(&mk, a.kv, a.kv.k, a.kv_heads)) return cudaErrorInvalidValue;
     // splits: two rounds of CTAs for every SM's four places, if each still has a few tiles of q
     const int tiles = (a.kv.max_len + AT_N - 1) / AT_N, nq = (a.max_rows + per - 1) / per;
+    if (tiles > 65535 || 16ll * a.kv_heads * a.seqs > 0x7fffffff) return cudaErrorInvalidValue;
     int split = 1;
     while (split < WT_MAX_SPLIT && (long long)tiles * a.kv_heads * a.seqs * split < 2ll * AT_SMS * WT_PER_SM && nq > 2 * split) split *= 2;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(tiles * split, a.kv_heads, a.seqs);
+    cfg.gridDim = dim3(split * a.kv_heads * a.seqs, tiles);
     cfg.blockDim = dim3(WT_THREADS);
     cfg.dynamicSmemBytes = WT_SMEM;
     cfg.stream = s;
