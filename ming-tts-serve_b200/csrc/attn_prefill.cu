@@ -143,6 +143,16 @@ struct PfRows {
 //    a warp of its own zeroes the values of positions that no row of the item
 //    sees (a weight of zero times a stale NaN would be NaN) before a block is
 //    handed to the products.
+// Bound by the exponentials: 16 results a cycle and SM are 1024 cycles for a
+// tile's 128 x 128 weights, twice its products' 550. Measured: 16 prompts of
+// 2048 rows (14 query, 2 kv heads, causal) 191 us, 629 TFLOP/s, the
+// exponential unit 62% busy, the tensor pipe 31%, a block of both tiles 2570
+// cycles; one prompt of 128 rows 7.3 us, all latency. Tried and slower at that
+// size: a polynomial on the multiply-add pipes for a quarter of the weights
+// (218 us against 200), two threads a row (250), weights against the maximum
+// so far with a second pass where it rose (247), unrolled code beyond one body
+// of 128 columns (the instruction cache; 297), 208 registers for the softmax
+// warps by setmaxnreg (spills; 1010).
 __global__ void __launch_bounds__(PF_THREADS, 1)
     attn_prefill_kernel(const AttnOp a, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                         const __grid_constant__ CUtensorMap mv, int tiles, int nx) {

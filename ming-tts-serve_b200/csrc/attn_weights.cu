@@ -34,8 +34,13 @@ constexpr int WT_SMEM = 1024 + AT_TILE + WT_STAGES * AT_TILE + WT_STAGES * WT_LS
 // shared memory to the first ranks, which add them up rank by rank while the
 // others leave: no atomics, one order of sums.
 // Bound by the exponentials, 16 a cycle and SM, one per visible pair: four
-// CTAs share an SM (128 tensor memory columns and 55 KB each) and fill
-// each other's waits, so each keeps one buffer of logits and two tiles of q.
+// CTAs share an SM (128 tensor memory columns and 55 KB each) and fill each
+// other's waits, so each keeps one buffer of logits and two tiles of q.
+// Measured: 8 prompts of up to 2048 rows (14 query, 2 kv heads) 56.6 us, the
+// exponential unit 46% busy: at its rate inside the loop, but a CTA's start
+// (its first logits 3 us after launch) and end take a third of its time. One
+// prompt of 333 rows: 7.4 us. Slower: two tiles of positions a cluster, from
+// both ends (78 us), three CTAs an SM with three tiles of q each (63).
 __global__ void __launch_bounds__(WT_THREADS, WT_PER_SM)
     attn_weights_kernel(const AttnOp a, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, int split) {
     extern __shared__ __align__(16) uint8_t wt_raw[];

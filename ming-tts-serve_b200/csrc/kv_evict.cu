@@ -12,7 +12,7 @@ constexpr int EV_THREADS = 512;
 constexpr int EV_WARPS = EV_THREADS / 32;
 constexpr int EV_BITS = 11;                 // radix of the selection: three digits of 11, 11 and 10 bits
 constexpr int EV_BINS = 1 << EV_BITS;
-constexpr int EV_AHEAD = 2;                 // 16-byte loads a thread has in flight
+constexpr int EV_AHEAD = 2;                 // rows of which a thread has a piece in flight
 
 // Order-preserving key of a total: larger total, larger key. -0 counts as +0
 // and NaN as -infinity.
@@ -49,6 +49,9 @@ MING_DEV int ev_scan(int x, int lane) {  // inclusive
 //    later one reads, and the next batch is read meanwhile.
 // Bound by the kept rows' bytes in a batch of sequences, by the chain of
 // dependent loads (length, totals, three histograms, pages, rows) for one.
+// Measured (24 layers, 2 kv heads): 16 sequences of up to 4096 positions cut
+// to 1024 69.6 us, 4.6 TB/s; one of 777 cut to 512 9.9 us. K and V in CTAs of
+// their own: 76 us; 256 threads 73; one or four rows ahead 74 and 90.
 template <int PARTS>
 __global__ void __launch_bounds__(EV_THREADS, 2) kv_evict_kernel(const EvictOp a) {
     extern __shared__ int ev_list[];  // positions that stay, ascending (when some between do and some do not)
