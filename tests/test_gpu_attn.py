@@ -202,7 +202,7 @@ def check_decode(ctx, c):
             assert torch.equal(acc[other], c.acc0[other])
 
 
-HEADS = [(14, 2), (16, 2), (8, 8), (4, 2), (5, 1), (3, 1)]
+HEADS = [(14, 2), (16, 2), (8, 8), (4, 2), (5, 1), (3, 1), (4, 1), (12, 2)]
 
 PREFILL = [
     # lens, rows
@@ -316,6 +316,13 @@ def test_decode_long_and_sharp(ctx):
     check_decode(ctx, Case([70001], [1], 14, 2, 0, 0, seed=3))
     check_decode(ctx, Case([20000, 11], [1, 1], 14, 2, 9000, 16, seed=4))
     check_decode(ctx, Case([1000] * 3, [1] * 3, 14, 2, 0, 0, sharp=60.0, seed=5))
+
+
+@pytest.mark.parametrize("lens", [[131001], [60001] * 5, [20, 60001, 0, 33, 59990]])
+def test_decode_totals_of_caches_past_shared_memory(ctx, lens):
+    """Logits that no CTA's shared memory holds: the keys are read a second time."""
+    c = Case(lens, [1] * len(lens), 14, 2, 0, 0, seed=8, poison=False)
+    check_decode(ctx, c)
 
 
 def test_one_row_of_a_prompt_is_a_token(ctx):
@@ -435,6 +442,47 @@ def test_evict(ctx, lens, keep, sinks, recent, kind, place):
     assert torch.equal(k_to[~touched].view(torch.int16), rest[0][~touched].view(torch.int16))
     assert torch.equal(v_to[~touched].view(torch.int16), rest[1][~touched].view(torch.int16))
     assert torch.equal(acc_to[~written].view(torch.int32), rest[2][~written].view(torch.int32))
+
+
+@pytest.mark.parametrize("seqs,layers", [(1, 24), (2, 24), (8, 24), (5, 40)])
+@pytest.mark.parametrize("place", ["apart", "same"])
+def test_evict_many_heads(ctx, seqs, layers, place):
+    """From few heads (several CTAs each) to many (one), against a stable sort."""
+    kvh, keep, sinks, recent = 2, 300, 3, 50
+    g = torch.Generator().manual_seed(seqs)
+    lens = [900] + torch.randint(1, 900, (seqs - 1,), generator=g).tolist()
+    c = Case(lens, [1] * seqs, 14, kvh, layers=layers, poison=False, seed=seqs)
+    n = torch.tensor(lens, device="cuda")[:, None, None, None]
+    acc = totals((seqs, layers, kvh, 900), "spread", seqs) * (torch.rand(seqs, layers, kvh, 900, device="cuda") > 0.3)
+    j = torch.arange(900, device="cuda")
+    a = torch.where((j < sinks) | (j >= n - recent), math.inf, acc)
+    a = torch.where(j < n, a, -math.inf)
+    best = a.argsort(dim=-1, descending=True, stable=True)[..., :keep].sort(-1).values
+    best = torch.where(n <= keep, j[:keep].expand_as(best), best)
+    stay = j[:keep] < n.clamp(max=keep)
+    want_index = torch.where(stay, best, -1)
+    b, l, h, s = stay.expand_as(best).nonzero(as_tuple=True)
+    i = best[b, l, h, s]
+    src = c.bt.long()[b, i // PAGE]
+    wk, wv, wa = c.k[src, l, h, i % PAGE], c.v[src, l, h, i % PAGE], acc[b, l, h, i]
+    index = torch.empty(seqs, layers, kvh, keep, dtype=torch.int32, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    if place == "same":
+        k_to, v_to, bt_to, acc_to = c.k, c.v, c.bt, acc
+        ctx.kv_evict(c.cache, acc=acc, keep=keep, sinks=sinks, recent=recent, index=index, stream=stream)
+    else:
+        kd = (keep + PAGE - 1) // PAGE
+        pool = torch.zeros(seqs * kd, layers, 2, kvh, PAGE, HD, dtype=torch.bfloat16, device="cuda")
+        k_to, v_to, acc_to = pool[:, :, 0], pool[:, :, 1], torch.zeros(seqs, layers, kvh, keep, device="cuda")
+        bt_to = torch.arange(seqs * kd, dtype=torch.int32, device="cuda").view(seqs, kd)
+        ctx.kv_evict(c.cache, M.KvCache(k_to, v_to, bt_to, c.lens_t, keep), acc, acc_to, keep=keep, sinks=sinks, recent=recent,
+                     index=index, stream=stream)
+    torch.cuda.synchronize()
+    ctx.sync()
+    dst = bt_to.long()[b, s // PAGE]
+    assert torch.equal(index.long(), want_index)
+    assert torch.equal(k_to[dst, l, h, s % PAGE], wk) and torch.equal(v_to[dst, l, h, s % PAGE], wv)
+    assert torch.equal(acc_to[b, l, h, s], wa)
 
 
 def test_evict_without_totals(ctx):
