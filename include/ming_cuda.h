@@ -271,7 +271,10 @@ int ming_cuda_vae_decode(ming_ctx* ctx, const uint16_t* latents, int T, float* w
  * page_stride + layer * layer_stride + head * head_stride + slot *
  * slot_stride + dim; V alike. Pages hold 16 positions, heads have 64 dims
  * (contiguous), values are bf16. Strides count elements and are multiples
- * of 8; k and v are 16-byte aligned. */
+ * of 8; k and v are 16-byte aligned. What a call writes (out, lse, acc, the
+ * cache and totals that an eviction moves to, index) overlaps nothing else
+ * that it reads or writes, but where an eviction is in place, and no two of
+ * its elements share a place. */
 typedef struct ming_kv_cache {
     uint16_t* k;
     uint16_t* v;
@@ -339,8 +342,8 @@ int ming_cuda_attn_decode(ming_ctx* ctx, const ming_kv_cache* cache, const ming_
  * stayed, [seqs][layers][kv_heads][keep], -1 behind them. Each sequence then
  * holds min(len, keep) positions; lens is not written and to's is not read.
  * `to` may be `from` with acc_to = acc (in place); else the pages and totals
- * of the two do not overlap. A page shared by two sequences must not be
- * evicted in place. acc and acc_to may be NULL if keep = sinks + recent;
+ * of the two do not overlap. A page that is written belongs to one sequence
+ * alone. acc and acc_to may be NULL if keep = sinks + recent;
  * otherwise keep is at most 49152. */
 typedef struct ming_evict {
     int keep, sinks, recent;

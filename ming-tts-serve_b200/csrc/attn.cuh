@@ -1,8 +1,9 @@
 // attn.cuh — attention over bounded paged K/V caches and their eviction:
 // what the operators' kernels share (attn_decode.cu: one new token per
-// sequence; attn_prefill.cu: a prompt's rows, and the weights they gave;
-// kv_evict.cu: eviction by accumulated weight), and their launchers. The
-// host side (argument checks, the C entry points) is attn_api.cu.
+// sequence; attn_prefill.cu: a prompt's rows; attn_weights.cu: the weights
+// they gave; kv_evict.cu: eviction by accumulated weight), and their
+// launchers. The host side (argument checks, the C entry points) is
+// attn_api.cu.
 //
 // Row i of a sequence holding len positions, n of them the rows' own, sits at
 // position p = len - n + i and sees j <= p with j < sinks or j > p - window

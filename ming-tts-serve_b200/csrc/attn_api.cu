@@ -119,11 +119,20 @@ int attn_op(ming_ctx* c, const ming_kv_cache* kv, const ming_attn* f, bool promp
     return MING_OK;
 }
 
-int check_out(const ming_attn* f, bool rows) {
+int check_out(const ming_attn* f, int rows) {
     if (!f->out && rows) return fail(MING_ERR_INVALID, "out is null");
     if (misaligned(f->out, 16) || f->out_row_stride % 8 || f->out_head_stride % 8 || f->out_row_stride < 0 ||
         f->out_head_stride < 0)
         return fail(MING_ERR_INVALID, "out must be 16-byte aligned, its strides multiples of 8 elements and not negative");
+    if ((rows > 1 && !f->out_row_stride) || (f->heads > 1 && rows && !f->out_head_stride))
+        return fail(MING_ERR_INVALID, "out: the strides of rows and heads must not be 0");
+    return MING_OK;
+}
+
+// Sequences and heads add to their totals at the same time.
+int check_totals(const ming_kv_cache* kv, const ming_attn* f) {
+    if (f->acc && ((kv->seqs > 1 && !f->acc_seq_stride) || (kv->kv_heads > 1 && !f->acc_head_stride)))
+        return fail(MING_ERR_INVALID, "acc: the strides of sequences and heads must not be 0");
     return MING_OK;
 }
 
@@ -148,7 +157,7 @@ int ming_cuda_attn_prefill(ming_ctx* c, const ming_kv_cache* kv, const ming_attn
     AttnOp a;
     int rc = attn_op(c, kv, f, true, &a);
     if (rc) return rc;
-    if ((rc = check_out(f, a.rows != 0))) return rc;
+    if ((rc = check_out(f, a.rows))) return rc;
     if (f->acc) return fail(MING_ERR_INVALID, "acc must be null (ming_cuda_attn_weights adds a prompt's weights)");
     return launch(c, f->stream, "attn_prefill", launch_attn_prefill, a, !a.seqs || !a.max_rows);
 }
@@ -159,6 +168,7 @@ int ming_cuda_attn_weights(ming_ctx* c, const ming_kv_cache* kv, const ming_attn
     if (rc) return rc;
     if (!f->lse && a.rows) return fail(MING_ERR_INVALID, "lse is null");
     if (!f->acc) return fail(MING_ERR_INVALID, "acc is null");
+    if ((rc = check_totals(kv, f))) return rc;
     return launch(c, f->stream, "attn_weights", launch_attn_weights, a, !a.seqs || !a.max_rows || !a.kv.max_len);
 }
 
@@ -166,8 +176,9 @@ int ming_cuda_attn_decode(ming_ctx* c, const ming_kv_cache* kv, const ming_attn*
     AttnOp a;
     int rc = attn_op(c, kv, f, false, &a);
     if (rc) return rc;
-    if ((rc = check_out(f, a.rows != 0))) return rc;
+    if ((rc = check_out(f, a.rows))) return rc;
     if (f->lse) return fail(MING_ERR_INVALID, "lse must be null");
+    if ((rc = check_totals(kv, f))) return rc;
     return launch(c, f->stream, "attn_decode", launch_attn_decode, a, !a.seqs);
 }
 
@@ -192,6 +203,15 @@ int ming_cuda_kv_evict(ming_ctx* c, const ming_kv_cache* from, const ming_kv_cac
     if (f->acc && (f->acc_seq_stride < 0 || f->acc_layer_stride < 0 || f->acc_head_stride < 0 || f->acc_to_seq_stride < 0 ||
                    f->acc_to_layer_stride < 0 || f->acc_to_head_stride < 0))
         return fail(MING_ERR_INVALID, "acc: negative stride");
+    if (f->acc && ((to->seqs > 1 && !f->acc_to_seq_stride) || (to->layers > 1 && !f->acc_to_layer_stride) ||
+                   (to->kv_heads > 1 && !f->acc_to_head_stride)))
+        return fail(MING_ERR_INVALID, "acc_to: the strides of sequences, layers and heads must not be 0");
+    if ((to->pages > 1 && !to->page_stride) || (to->layers > 1 && !to->layer_stride) || (to->kv_heads > 1 && !to->head_stride))
+        return fail(MING_ERR_INVALID, "to: the strides of pages, layers and heads must not be 0");
+    if ((from->k == to->k || from->v == to->v) &&
+        (from->k != to->k || from->v != to->v || from->page_stride != to->page_stride || from->layer_stride != to->layer_stride ||
+         from->head_stride != to->head_stride || from->slot_stride != to->slot_stride))
+        return fail(MING_ERR_INVALID, "from and to are the same pool with other strides");
     if (f->acc == f->acc_to && f->acc &&
         (f->acc_seq_stride != f->acc_to_seq_stride || f->acc_layer_stride != f->acc_to_layer_stride ||
          f->acc_head_stride != f->acc_to_head_stride))

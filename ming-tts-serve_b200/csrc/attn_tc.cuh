@@ -94,14 +94,6 @@ MING_DEV void at_ld16(uint32_t* v, uint32_t addr) {
         : AT_R8(v, 0), AT_R8(v, 8)
         : "r"(addr));
 }
-MING_DEV void at_st32(uint32_t addr, const uint32_t* v) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(
-            addr),
-        AT_W8(v, 0), AT_W8(v, 8), AT_W8(v, 16), AT_W8(v, 24)
-        : "memory");
-}
 MING_DEV void at_st16(uint32_t addr, const uint32_t* v) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(addr),
@@ -166,7 +158,6 @@ MING_DEV void at_copy_q(void* dst, const CUtensorMap* m, int head, int row, uint
         "l"(reinterpret_cast<uint64_t>(m)), "r"(0), "r"(head), "r"(row), "r"(at_su32(bar))
         : "memory");
 }
-
 
 // Host: tensor maps
 constexpr int AT_SMS = 148;

@@ -219,7 +219,7 @@ cudaError_t launch_kv_evict(const EvictOp& a, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(a.kv_heads * parts, a.layers, a.seqs);
     cfg.blockDim = dim3(EV_THREADS);
-    cfg.dynamicSmemBytes = a.sinks + a.recent < a.keep ? (size_t)a.keep * 4 : 0;
+    cfg.dynamicSmemBytes = a.sinks + a.recent < a.keep && a.keep < a.from.max_len ? (size_t)a.keep * 4 : 0;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;

@@ -262,6 +262,7 @@ class KvCache:
         self.k, self.v, self.block_table, self.lens, self.max_len = k, v, block_table, lens, int(max_len)
         self.seqs, self.shape = lens.shape[0], (lens.shape[0], k.shape[1], k.shape[2])
         _want(0 <= self.max_len <= 16 * block_table.shape[1], "max_len does not fit the block table")
+        _want(self.seqs < 2 or st[0] >= block_table.shape[1], "block_table: rows of their own are wanted")
         self.args = KvCacheArgs(k.data_ptr(), v.data_ptr(), s[0], s[1], s[2], s[3], k.shape[0], k.shape[1], k.shape[2],
                                 self.seqs, block_table.data_ptr(), st[0] or block_table.shape[1], self.max_len,
                                 lens.data_ptr())
@@ -538,6 +539,7 @@ class Context:
         index: int32 [seqs, layers, kv_heads, keep] or None. The sequences
         then hold min(len, keep) positions (lens is the caller's to update)."""
         if to is None:
+            _want(acc_to is None or acc_to is acc, "acc_to goes with another cache")
             to, acc_to = cache, acc
         if cache.device != self.device or to.device != self.device:
             raise MingError("the cache is on another device")

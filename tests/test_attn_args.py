@@ -46,7 +46,7 @@ def call(name, c, a):
     return getattr(M.lib(), "ming_cuda_attn_" + name)(None, ctypes.byref(c) if c else None, ctypes.byref(a) if a else None)
 
 
-OPS = {"prefill": {}, "weights": dict(lse=AT, acc=AT), "decode": {}}
+OPS = {"prefill": {}, "weights": dict(lse=AT, acc=AT, acc_seq_stride=256, acc_head_stride=128), "decode": {}}
 
 
 @pytest.mark.parametrize("op", OPS)
@@ -107,6 +107,20 @@ def test_a_prompt_steps_over_its_strides(op, c, a):
         refused(call("decode", cache(), attn(**a)), "null context")
 
 
+@pytest.mark.parametrize("op,bad,word", [
+    ("prefill", dict(out_row_stride=0), "out: the strides"), ("prefill", dict(out_head_stride=0), "out: the strides"),
+    ("decode", dict(out_row_stride=0), "out: the strides"), ("decode", dict(out_head_stride=0), "out: the strides"),
+    ("weights", dict(acc_seq_stride=0), "acc: the strides"), ("weights", dict(acc_head_stride=0), "acc: the strides"),
+    ("decode", dict(acc=AT, acc_head_stride=128), "acc: the strides"),
+    ("decode", dict(acc=AT, acc_seq_stride=256), "acc: the strides"),
+])
+def test_results_have_places_of_their_own(op, bad, word):
+    refused(call(op, cache(), attn(**{**OPS[op], **bad})), word, "must not be 0")
+    # nothing to step over: one sequence, one row, one head
+    one = dict(heads=1, rows=1, max_rows=1)
+    refused(call(op, cache(seqs=1, kv_heads=1), attn(**{**OPS[op], **one, **bad})), "null context")
+
+
 def test_null_structures():
     for op in OPS:
         refused(call(op, None, attn()), "null")
@@ -124,6 +138,11 @@ def test_null_structures():
     (dict(), dict(sinks=20, recent=13), "fit in keep"), (dict(), dict(sinks=2**31 - 1, recent=2**31 - 1), "fit in keep"),
     (dict(bt_ld=1, max_len=16), dict(), "does not fit to's"), (dict(), dict(acc=0, acc_to=0), "acc is null"),
     (dict(), dict(acc_to=0), "go together"), (dict(), dict(acc=0, sinks=24), "go together"), (dict(), dict(index=AT + 2), "4-byte"),
+    (dict(page_stride=0), dict(), "to: the strides"), (dict(head_stride=0), dict(), "to: the strides"),
+    (dict(k=AT + 128), dict(), "same pool"), (dict(v=AT + 128), dict(), "same pool"), (dict(slot_stride=128), dict(), "same pool"),
+    (dict(page_stride=8192), dict(), "same pool"), (dict(k=AT + 128, v=AT + 128, slot_stride=128), dict(), "null context"),
+    (dict(), dict(acc_to_seq_stride=0), "acc_to: the strides"), (dict(), dict(acc_to_head_stride=0), "acc_to: the strides"),
+    (dict(), dict(acc_seq_stride=0, acc_head_stride=0), "null context"),  # shared totals may be read
     (dict(bt_ld=9999, max_len=159984), dict(keep=49153), "at most 49152"), (dict(), dict(acc_to_seq_stride=-1), "negative"), (dict(), dict(acc_to=AT, acc_to_head_stride=64), "other strides"),
 ])
 def test_evict_arguments(to, bad, word):

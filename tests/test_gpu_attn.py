@@ -668,6 +668,30 @@ def test_refusals_of_the_python_layer(ctx):
             pytest.fail(f"call {i} was accepted")
 
 
+def test_broadcast_tensors_are_refused(ctx):
+    """A table whose rows are one row, results and totals that share places."""
+    c = Case([40, 40], [1, 1], 14, 2)
+    o = torch.empty_like(c.q)
+    to = M.KvCache(c.k.clone(), c.v.clone(), c.bt, c.lens_t, 40)
+    bad = [
+        lambda: M.KvCache(c.k, c.v, c.bt[:1].expand(2, -1), c.lens_t, 40),
+        lambda: M.KvCache(c.k, c.v, c.bt[:1, :1].expand(2, 1), c.lens_t, 16),
+        lambda: M.KvCache(c.k, c.v, c.bt, c.lens_t[:1].expand(2), 40),
+        lambda: ctx.attn_prefill(c.q, c.q_start, c.cache, o[:1].expand_as(o)),
+        lambda: ctx.attn_decode(c.q, c.cache, o[:, :1].expand_as(o)),
+        lambda: ctx.attn_decode(c.q, c.cache, o, acc=c.acc0[:1].expand_as(c.acc0)),
+        lambda: ctx.attn_weights(c.q, c.q_start, c.cache, torch.zeros(2, 14, device="cuda"), c.acc0[:, :, :1].expand_as(c.acc0)),
+        lambda: ctx.kv_evict(c.cache, to, c.acc0, c.acc0[:1].expand_as(c.acc0), keep=20),
+        lambda: ctx.kv_evict(c.cache, None, c.acc0, c.acc0.clone(), keep=20),
+    ]
+    for i, f in enumerate(bad):
+        with pytest.raises(M.MingError):
+            f()
+            pytest.fail(f"call {i} was accepted")
+    # a batch of one has nothing to step over
+    M.KvCache(c.k, c.v, c.bt[:1].expand(1, -1), c.lens_t[:1], 40)
+
+
 def test_nothing_to_do(ctx):
     s = torch.cuda.current_stream().cuda_stream
     c = Case([40, 9], [0, 0], 14, 2, poison=False)
