@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "attn.cuh"
 
@@ -15,9 +16,9 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int DE_MAX_SPLIT = 16;          // CTAs of a cluster
-constexpr int DE_OLD = AT_HD + 4;         // row of merged outputs: float4-aligned, rows on other banks
-constexpr int de_part(int warps) { return warps * AT_MAXG * (DE_OLD + 2); }  // floats: every warp's outputs, maxima and sums
-constexpr int de_smem(int warps) { return (de_part(warps) + AT_MAXG * (DE_OLD + 2) + 2 * AT_MAXG) * 4; }
+constexpr int de_old(int dims) { return dims + 4; }  // row of merged outputs: float4-aligned, rows on other banks
+constexpr int de_part(int warps, int dims) { return warps * AT_MAXG * (de_old(dims) + 2); }  // floats: every warp's outputs, maxima and sums
+constexpr int de_smem(int warps, int dims) { return (de_part(warps, dims) + AT_MAXG * (de_old(dims) + 2) + 2 * AT_MAXG) * 4; }
 constexpr int DE_SMEM_MAX = 200 * 1024;
 
 enum { DE_PLAIN = 0, DE_TRACK = 1, DE_TRACK_AGAIN = 2 };
@@ -41,7 +42,8 @@ struct SeenPages {
 MING_DEV uint32_t de_prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
 }  // namespace
 
-// A cluster per (sequence, kv head); its CTAs split the row's pages, a CTA's
+// Clusters of a (sequence, kv head), PARTS of them, take a part of the values'
+// dims each and all of the keys; a cluster's CTAs split the row's pages, a CTA's
 // warps take them in turn. Per page of 16 positions a warp runs the group's
 // heads (8 of the 16 rows of mma.sync m16n8k16; one token has too few rows for
 // the 128-row tensor-memory instructions) against keys and values that come
@@ -50,9 +52,10 @@ MING_DEV uint32_t de_prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_
 //    takes bytes [16 t, 16 t + 16) and [64 + 16 t, ..) of position g's row,
 //    two 16-byte loads, and q's fragments are permuted alike;
 //  * output columns may carry any dim, so lane (g, t) of a value fragment
-//    takes bytes [16 g, 16 g + 16) of rows 2t, 2t+1, 2t+8, 2t+9; column tile
-//    i then holds dims 8 c + i of its columns c, and a lane ends up with 16
-//    consecutive dims of one head.
+//    takes bytes [16 g, 16 g + 16) of rows 2t, 2t+1, 2t+8, 2t+9 (8 or 4 bytes
+//    where PARTS clusters share the dims); column tile i then holds dims 8 c +
+//    i of its columns c, and a lane ends up with 16 consecutive dims of one
+//    head.
 // The next page's eight loads are issued before the current one's products:
 // 4 KB in flight per warp, nothing staged in shared memory. Weights enter the
 // second product as bf16 hi in rows 0-7 and lo in rows 8-15 (the rows that the
@@ -64,27 +67,29 @@ MING_DEV uint32_t de_prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_
 // DE_TRACK keeps the logits in shared memory until the join, DE_TRACK_AGAIN
 // (longer than fits) reads the keys a second time.
 // Bound by: the cache's bytes (256 per position and kv head) for batches, the
-// launch, two dependent loads and the cluster's two barriers for short rows.
-// Measured (14 query, 2 kv heads): 64 x 4096 positions 28.6 us, 4.7 TB/s, and
-// 38.0 us with tracking (its logits take the L1's room from the loads in
-// flight); 1 x 509 5.0 us; 1 x 32768 16.0 us: a cluster sits in one part of
-// the chip, whose share of the memory's rate is an eighth, so two heads alone
-// cannot have all of it. Rings of cp.async three pages ahead and operands
-// swapped for half the products changed none of this (34, 42 and 18 us).
-template <int MODE, int WARPS>
+// launch, two dependent loads and the cluster's two barriers for short rows,
+// what one SM takes in (some 65 GB/s) for few heads.
+// Measured (14 query, 2 kv heads): 64 x 4096 positions 27.9 us, 4.8 TB/s, and
+// 37.1 us with tracking (its logits take the L1's room from the loads in
+// flight); 1 x 509 4.2 us; 1 x 32768 10.3 us. Rings of cp.async three pages
+// ahead and operands swapped for half the products changed none of this (34,
+// 42 and 18 us against 29, 38 and 16 at the time).
+template <int MODE, int WARPS, int PARTS>
 __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) attn_decode_kernel(const AttnOp a, int sc_ld) {
-    constexpr int THREADS = WARPS * 32;
+    constexpr int THREADS = WARPS * 32, DIMS = AT_HD / PARTS, NT = DIMS / 8;  // output dims of a cluster, column tiles
+    constexpr int DE_OLD = de_old(DIMS);
+    static_assert(PARTS == 1 || PARTS == 2 || PARTS == 4, "a lane's values of a row are 16, 8 or 4 bytes");
     extern __shared__ __align__(16) float de_buf[];
     float* wo = de_buf;                                  // [warp][head][DE_OLD]
     float* wm = wo + WARPS * AT_MAXG * DE_OLD;        // [warp][head]
     float* wl = wm + WARPS * AT_MAXG;
-    float* co = de_buf + de_part(WARPS);                       // this CTA's [head][DE_OLD], unnormalised
+    float* co = de_buf + de_part(WARPS, DIMS);                 // this CTA's [head][DE_OLD], unnormalised
     float* cm = co + AT_MAXG * DE_OLD;
     float* cl = cm + AT_MAXG;
     float* fm = cl + AT_MAXG;                            // the cluster's maxima and 1 / sums
     float* fl = fm + AT_MAXG;
     float* sc = fl + AT_MAXG;                            // DE_TRACK: logits [head][sc_ld]
-    const int rank = blockIdx.x, ns = gridDim.x, kh = blockIdx.y, b = blockIdx.z;
+    const int rank = blockIdx.x, ns = gridDim.x, kh = blockIdx.y / PARTS, part = blockIdx.y % PARTS, b = blockIdx.z;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int seq = at_seq(a.kv, b);
     const int* bt = a.kv.bt + (size_t)seq * a.kv.bt_ld;
@@ -100,9 +105,9 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) attn_decode_kernel(con
         qa[0][0] = has ? x.x : 0u, qa[1][0] = has ? x.y : 0u, qa[2][0] = has ? x.z : 0u, qa[3][0] = has ? x.w : 0u;
         qa[0][1] = has ? y.x : 0u, qa[1][1] = has ? y.y : 0u, qa[2][1] = has ? y.z : 0u, qa[3][1] = has ? y.w : 0u;
     }
-    float m = -INFINITY, l = 0.f, o[8][4];
+    float m = -INFINITY, l = 0.f, o[NT][4];
 #pragma unroll
-    for (int i = 0; i < 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    for (int i = 0; i < NT; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 
     // this warp's pages: v0 + warp, + 8, ..; a lane looks up every 32nd ahead of use
     const int first = v0 + warp, count = first < v1 ? (v1 - first + WARPS - 1) / WARPS : 0;
@@ -111,7 +116,9 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) attn_decode_kernel(con
         const int i = i0 + lane;
         ids = i < count ? at_page(a.kv, bt, see.page(first + i * WARPS), a.err) : 0;
     };
-    uint4 kf[4], vf[4];  // the page in flight
+    using Vals = std::conditional_t<PARTS == 1, uint4, std::conditional_t<PARTS == 2, uint2, uint32_t>>;  // a lane's values of a row
+    uint4 kf[4];  // the page in flight
+    Vals vf[4];
     auto fetch_k = [&](int64_t base) {
         const uint16_t* r0 = a.kv.k + base + g * a.kv.ss + 8 * t;
         const uint16_t* r8 = r0 + 8 * a.kv.ss;
@@ -121,11 +128,13 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) attn_decode_kernel(con
         kf[3] = ldg_nc16(r8 + 32);
     };
     auto fetch_v = [&](int64_t base) {
-        const uint16_t* r0 = a.kv.v + base + 2 * t * a.kv.ss + 8 * g;
-        vf[0] = ldg_nc16(r0);
-        vf[1] = ldg_nc16(r0 + a.kv.ss);
-        vf[2] = ldg_nc16(r0 + 8 * a.kv.ss);
-        vf[3] = ldg_nc16(r0 + 9 * a.kv.ss);
+        const uint16_t* r0 = a.kv.v + base + 2 * t * a.kv.ss + part * DIMS + NT * g;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint16_t* r = r0 + ((i >> 1) * 8 + (i & 1)) * a.kv.ss;
+            if constexpr (PARTS == 1) vf[i] = ldg_nc16(r);
+            else vf[i] = __ldg(reinterpret_cast<const Vals*>(r));
+        }
     };
     auto base_of = [&](int i) { return (int64_t)__shfl_sync(0xffffffffu, ids, i & 31) * a.kv.ps + kh * a.kv.hs; };
     // logits of the page in kf: c[0..1] positions 2t, 2t+1, c[2..3] positions 8 + 2t, ..
@@ -157,7 +166,8 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) attn_decode_kernel(con
     }
     for (int i = 0; i < count; i++) {
         const int vi = first + i * WARPS, p = see.page(vi);
-        uint4 k[4] = {kf[0], kf[1], kf[2], kf[3]}, v[4] = {vf[0], vf[1], vf[2], vf[3]};
+        uint4 k[4] = {kf[0], kf[1], kf[2], kf[3]};
+        Vals v[4] = {vf[0], vf[1], vf[2], vf[3]};
         if (i + 1 < count) {
             if (((i + 1) & 31) == 0) look_up(i + 1);
             const int64_t base = base_of(i + 1);
@@ -166,17 +176,17 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) attn_decode_kernel(con
         }
         float c[4];
         logits(k, p, c);
-        if (MODE == DE_TRACK) {
+        if (MODE == DE_TRACK && part == 0) {
             float* s = sc + g * sc_ld + (vi - v0) * AT_PAGE + 2 * t;
             *reinterpret_cast<float2*>(s) = make_float2(c[0], c[1]);
             *reinterpret_cast<float2*>(s + 8) = make_float2(c[2], c[3]);
         }
         if (!see.whole(p)) {  // 0 x NaN is NaN: values that are not seen become zeros
             const int j = p * AT_PAGE + 2 * t;
-            if (!see.sees(j)) v[0] = make_uint4(0, 0, 0, 0);
-            if (!see.sees(j + 1)) v[1] = make_uint4(0, 0, 0, 0);
-            if (!see.sees(j + 8)) v[2] = make_uint4(0, 0, 0, 0);
-            if (!see.sees(j + 9)) v[3] = make_uint4(0, 0, 0, 0);
+            if (!see.sees(j)) v[0] = Vals{};
+            if (!see.sees(j + 1)) v[1] = Vals{};
+            if (!see.sees(j + 8)) v[2] = Vals{};
+            if (!see.sees(j + 9)) v[3] = Vals{};
         }
         float mx = fmaxf(fmaxf(c[0], c[1]), fmaxf(c[2], c[3]));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -186,7 +196,7 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) attn_decode_kernel(con
             m = mn;
             l *= r;
 #pragma unroll
-            for (int d = 0; d < 8; d++) o[d][0] *= r, o[d][1] *= r, o[d][2] *= r, o[d][3] *= r;
+            for (int d = 0; d < NT; d++) o[d][0] *= r, o[d][1] *= r, o[d][2] *= r, o[d][3] *= r;
         }
         float e[4];
 #pragma unroll
@@ -195,15 +205,20 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) attn_decode_kernel(con
         const uint32_t h0 = at_bf16x2(e[0], e[1]), h1 = at_bf16x2(e[2], e[3]);
         const float2 f0 = unpack_bf16x2(h0), f1 = unpack_bf16x2(h1);
         const uint32_t pa[4] = {h0, at_bf16x2(e[0] - f0.x, e[1] - f0.y), h1, at_bf16x2(e[2] - f1.x, e[3] - f1.y)};
-        const uint32_t vw[4][4] = {{v[0].x, v[1].x, v[2].x, v[3].x}, {v[0].y, v[1].y, v[2].y, v[3].y},
-                                   {v[0].z, v[1].z, v[2].z, v[3].z}, {v[0].w, v[1].w, v[2].w, v[3].w}};
+        uint32_t vw[NT / 2][4];  // [two column tiles][row]
 #pragma unroll
-        for (int d = 0; d < 4; d++) {
+        for (int r = 0; r < 4; r++) {
+            if constexpr (PARTS == 1) vw[0][r] = v[r].x, vw[1][r] = v[r].y, vw[2][r] = v[r].z, vw[3][r] = v[r].w;
+            else if constexpr (PARTS == 2) vw[0][r] = v[r].x, vw[1][r] = v[r].y;
+            else vw[0][r] = v[r];
+        }
+#pragma unroll
+        for (int d = 0; d < NT / 2; d++) {
             mma_bf16(o[2 * d], pa, de_prmt(vw[d][0], vw[d][1], 0x5410), de_prmt(vw[d][2], vw[d][3], 0x5410));
             mma_bf16(o[2 * d + 1], pa, de_prmt(vw[d][0], vw[d][1], 0x7632), de_prmt(vw[d][2], vw[d][3], 0x7632));
         }
     }
-    // the warp's part: lane (g, t) holds dims 16 t .. 16 t + 15 of head g
+    // the warp's part: lane (g, t) holds dims 2 NT t .. 2 NT t + 2 NT - 1 of head g
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     if (t == 0) {
@@ -211,32 +226,37 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) attn_decode_kernel(con
         wl[warp * AT_MAXG + g] = l;
     }
     {
-        float* w = wo + (warp * AT_MAXG + g) * DE_OLD + 16 * t;
+        float* w = wo + (warp * AT_MAXG + g) * DE_OLD + 2 * NT * t;
+        float x[2 * NT];
 #pragma unroll
         for (int c = 0; c < 2; c++)
 #pragma unroll
-            for (int d = 0; d < 8; d += 4)
-                *reinterpret_cast<float4*>(w + 8 * c + d) = make_float4(o[d][c] + o[d][c + 2], o[d + 1][c] + o[d + 1][c + 2],
-                                                                        o[d + 2][c] + o[d + 2][c + 2], o[d + 3][c] + o[d + 3][c + 2]);
+            for (int d = 0; d < NT; d++) x[NT * c + d] = o[d][c] + o[d][c + 2];
+#pragma unroll
+        for (int d = 0; d < 2 * NT; d += 4) *reinterpret_cast<float4*>(w + d) = make_float4(x[d], x[d + 1], x[d + 2], x[d + 3]);
     }
     __syncthreads();
-    // the CTA's part: eight warps a head each, or sixteen half a head
-    {
-        constexpr int DIMS = 16 / WARPS;  // a lane's
-        const int h = warp % AT_MAXG, d0 = (warp / AT_MAXG) * 32 + DIMS * lane;
-        float M = -INFINITY, L = 0.f, x[DIMS] = {};
+    // the CTA's part: the lanes of a head look at a warp's maximum each
+    constexpr int OWN = AT_MAXG * DIMS > THREADS ? AT_MAXG * DIMS / THREADS : 1;  // a thread's dims
+    static_assert(DIMS / OWN >= WARPS, "a head's lanes are fewer than the warps");
+    if (tid * OWN < AT_MAXG * DIMS) {
+        const int h = tid * OWN / DIMS, d0 = tid * OWN % DIMS, at = (lane % WARPS) * AT_MAXG + h;
+        float M = wm[at];
 #pragma unroll
-        for (int w = 0; w < WARPS; w++) M = fmaxf(M, wm[w * AT_MAXG + h]);
+        for (int i = 1; i < WARPS; i <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, i));
+        const float f = M == -INFINITY ? 0.f : exp2f(wm[at] - M);
+        float L = wl[at] * f, x[OWN] = {};
+#pragma unroll
+        for (int i = 1; i < WARPS; i <<= 1) L += __shfl_xor_sync(0xffffffffu, L, i);
 #pragma unroll
         for (int w = 0; w < WARPS; w++) {
-            const float f = M == -INFINITY ? 0.f : exp2f(wm[w * AT_MAXG + h] - M);
-            L += wl[w * AT_MAXG + h] * f;
+            const float fw = __shfl_sync(0xffffffffu, f, w, WARPS);
 #pragma unroll
-            for (int d = 0; d < DIMS; d++) x[d] += wo[(w * AT_MAXG + h) * DE_OLD + d0 + d] * f;
+            for (int d = 0; d < OWN; d++) x[d] += wo[(w * AT_MAXG + h) * DE_OLD + d0 + d] * fw;
         }
 #pragma unroll
-        for (int d = 0; d < DIMS; d++) co[h * DE_OLD + d0 + d] = x[d];
-        if (lane == 0 && warp < AT_MAXG) cm[h] = M, cl[h] = L;
+        for (int d = 0; d < OWN; d++) co[h * DE_OLD + d0 + d] = x[d];
+        if (d0 == 0) cm[h] = M, cl[h] = L;
     }
     // the totals that this thread adds to, on their way while the parts meet
     float* const acc = MODE == DE_TRACK ? a.acc + seq * a.a_ss + kh * a.a_hs : nullptr;
@@ -250,37 +270,61 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) attn_decode_kernel(con
             old[k] = see.sees(j) && j != see.n - 1 ? acc[j] : 0.f;
         }
     };
-    if (MODE == DE_TRACK) fetch_acc(tid);
+    if (MODE == DE_TRACK && part == 0) fetch_acc(tid);
     cg::cluster_group cluster = cg::this_cluster();
     if (ns > 1) cluster.sync();
     else __syncthreads();
-    // the cluster's: the group's outputs, two dims at a time, over the ranks
-    for (int e = rank * THREADS + tid; e < a.group * (AT_HD / 2); e += ns * THREADS) {
-        const int h = e / (AT_HD / 2), d = e % (AT_HD / 2);
-        float M = -INFINITY, L = 0.f, x = 0.f, y = 0.f;
-        for (int r = 0; r < ns; r++) M = fmaxf(M, ns > 1 ? *cluster.map_shared_rank(cm + h, r) : cm[h]);
-        for (int r = 0; r < ns; r++) {
-            const float* po = ns > 1 ? cluster.map_shared_rank(co, r) : co;
-            const float f = M == -INFINITY ? 0.f : exp2f(po[AT_MAXG * DE_OLD + h] - M);
-            const float2 v = *reinterpret_cast<const float2*>(po + h * DE_OLD + 2 * d);
-            L += po[AT_MAXG * DE_OLD + AT_MAXG + h] * f;
-            x += v.x * f;
-            y += v.y * f;
-        }
-        const float il = L > 0.f ? 1.f / L : 0.f;
-        reinterpret_cast<uint32_t*>(a.out + b * a.o_rs + (kh * a.group + h) * a.o_hs)[d] = at_bf16x2(x * il, y * il);
-    }
-    if (MODE != DE_PLAIN) {
-        if (tid < AT_MAXG) {
-            float M = -INFINITY, L = 0.f;
-            for (int r = 0; r < ns; r++) M = fmaxf(M, ns > 1 ? *cluster.map_shared_rank(cm + tid, r) : cm[tid]);
-            for (int r = 0; r < ns; r++) {
-                const float* pm = ns > 1 ? cluster.map_shared_rank(cm, r) : cm;
-                L += M == -INFINITY ? 0.f : pm[AT_MAXG + tid] * exp2f(pm[tid] - M);
+    // The cluster's: the group's outputs, two dims at a time, and the heads'
+    // maxima and sums. Every rank is asked at once, one trip to the others'
+    // shared memory (a loop over sixteen ranks took 1.5 us).
+    auto join = [&](auto ranks) {
+        constexpr int N = decltype(ranks)::value;  // at least ns
+        float f[N], M, L;
+        auto sums = [&](int h) {
+            float l[N];
+#pragma unroll
+            for (int r = 0; r < N; r++) {
+                const float* p = N > 1 && r < ns ? cluster.map_shared_rank(cm + h, r) : cm + h;
+                f[r] = r < ns ? p[0] : -INFINITY;
+                l[r] = r < ns ? p[AT_MAXG] : 0.f;
             }
+            M = f[0], L = 0.f;
+#pragma unroll
+            for (int r = 1; r < N; r++) M = fmaxf(M, f[r]);
+#pragma unroll
+            for (int r = 0; r < N; r++) {
+                f[r] = M == -INFINITY ? 0.f : exp2f(f[r] - M);
+                L += l[r] * f[r];
+            }
+        };
+        for (int e = rank * THREADS + tid; e < a.group * (DIMS / 2); e += ns * THREADS) {
+            const int h = e / (DIMS / 2), d = e % (DIMS / 2);
+            float2 v[N];
+#pragma unroll
+            for (int r = 0; r < N; r++) {
+                const float* p = co + h * DE_OLD + 2 * d;
+                v[r] = r < ns ? *reinterpret_cast<const float2*>(N > 1 ? cluster.map_shared_rank(p, r) : p) : make_float2(0.f, 0.f);
+            }
+            sums(h);
+            float x = 0.f, y = 0.f;
+#pragma unroll
+            for (int r = 0; r < N; r++) {
+                x += v[r].x * f[r];
+                y += v[r].y * f[r];
+            }
+            const float il = L > 0.f ? 1.f / L : 0.f;
+            reinterpret_cast<uint32_t*>(a.out + b * a.o_rs + (kh * a.group + h) * a.o_hs + part * DIMS)[d] = at_bf16x2(x * il, y * il);
+        }
+        if (MODE != DE_PLAIN && part == 0 && tid < AT_MAXG) {
+            sums(tid);
             fm[tid] = M;
             fl[tid] = L > 0.f ? 1.f / L : 0.f;
         }
+    };
+    if (ns == 1) join(std::integral_constant<int, 1>());
+    else if (ns <= 4) join(std::integral_constant<int, 4>());
+    else join(std::integral_constant<int, DE_MAX_SPLIT>());
+    if (MODE != DE_PLAIN && part == 0) {
         __syncthreads();
         if (MODE == DE_TRACK) {
             for (int e0 = tid; e0 < mine; e0 += 4 * THREADS) {
@@ -324,16 +368,81 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) attn_decode_kernel(con
     if (ns > 1) cluster.sync();  // the others may still be reading this CTA's part
 }
 
+namespace {
+using DeKernel = void (*)(AttnOp, int);
+template <int WARPS, int PARTS>
+DeKernel de_kernel(int mode) {
+    if (mode == DE_PLAIN) return attn_decode_kernel<DE_PLAIN, WARPS, PARTS>;
+    if (mode == DE_TRACK) return attn_decode_kernel<DE_TRACK, WARPS, PARTS>;
+    if constexpr (WARPS == 16 || PARTS == 1) return attn_decode_kernel<DE_TRACK_AGAIN, WARPS, PARTS>;
+    else return nullptr;  // so many heads are not divided by dims
+}
+DeKernel de_kernel(int warps, int parts, int mode) {
+    return warps == 8 ? parts == 1 ? de_kernel<8, 1>(mode) : parts == 2 ? de_kernel<8, 2>(mode) : de_kernel<8, 4>(mode)
+                      : parts == 1 ? de_kernel<16, 1>(mode) : parts == 2 ? de_kernel<16, 2>(mode) : de_kernel<16, 4>(mode);
+}
+
+// How a launch is divided: CTAs of a cluster, which split the pages; clusters
+// of a head, which share the values' dims; warps of a CTA; the mode and its
+// shared memory.
+struct DePlan {
+    int ns, parts, warps, mode, ld;
+    size_t smem;
+};
+
+// An SM takes in about 4 KB in 0.06 us, however many loads are in flight, so
+// few heads want many SMs: the pages are split, and then the dims (each
+// cluster reads all keys and its part of the values). The plan of the least
+// cost in pages of that rate is taken:
+//   (pages of a CTA, at least one a warp) x (1 + 1 / parts) / 2, twice if the keys are read again
+//   x 1.8 per two CTAs on an SM
+//   + 8 + 0.8 ns for a cluster's barriers and join, + 12 for outputs of all 64 dims.
+// Fitted to 80 shapes (1 to 64 sequences, 128 to 32768 positions, tracked and
+// not, 2 kv heads) of 6 to 25 plans each: the one taken is 0.7% behind the
+// best on average. 1 x 32768 positions: 10.6 us in 2 x 16 CTAs a head, 15.0 in
+// 1 x 16, 14.6 in 4 x 8; 1 x 509: 4.3 in 4 x 4, 4.9 in 1 x 8; 32 x 509: 5.4 in
+// 2 x 1, 6.5 in 1 x 2; 64 x 4096: 28.6 in 1 x 2, 34 in 1 x 4, 42 in 1 x 1.
+// Sixteen warps a CTA pay where the SM has no other and each gets more than a page.
+DePlan de_plan(long long heads, long long pages, bool track) {
+    // clusters find place within one part of the chip: fewer of the large ones
+    constexpr int sms[5] = {148, 148, 144, 120, 112};
+    DePlan best{};
+    double least = 0;
+    for (int i = 0; i < 5; i++)
+        for (int parts = 1; parts <= 4; parts *= 2) {
+            const int ns = 1 << i;
+            const long long ctas = heads * ns * parts;
+            const bool alone = ctas <= sms[i];
+            if (ns == DE_MAX_SPLIT && !alone) continue;
+            DePlan p{ns, parts, alone && pages > 16 * ns ? 16 : 8, DE_PLAIN, 0, 0};
+            p.smem = de_smem(p.warps, AT_HD / parts);
+            bool two = true;
+            if (track) {
+                const long long ld = (pages + ns - 1) / ns * AT_PAGE / 32 * 32 + 40;  // 8 past a multiple of 32: the eight heads' stores fall on distinct banks
+                const size_t smem = p.smem + ld * AT_MAXG * 4;
+                p.mode = smem <= DE_SMEM_MAX ? DE_TRACK : DE_TRACK_AGAIN;
+                if (p.mode == DE_TRACK_AGAIN && p.warps == 8 && parts > 1) continue;
+                if (p.mode == DE_TRACK) p.ld = (int)ld, p.smem = smem, two = smem <= 112 * 1024;
+            }
+            const long long slots = two ? 2 * sms[i] : sms[i];
+            const double share = alone ? 1. : (two ? 1.8 : 1.) * (double)((ctas + slots - 1) / slots);
+            const double cost = std::max((double)pages / ns, 8.) * (1. + 1. / parts) / 2 * share * (p.mode == DE_TRACK_AGAIN ? 2 : 1) +
+                                (ns > 1 ? 8 + 0.8 * ns : 0.) + (parts == 1 ? 12. : 0.);
+            if (best.ns == 0 || cost < least) best = p, least = cost;
+        }
+    return best;
+}
+}  // namespace
+
 cudaError_t launch_attn_decode(const AttnOp& a, cudaStream_t s) {
     static std::atomic<bool> ready[64] = {};  // per device: the kernels' attributes are set
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {
-        const void* f[6] = {(const void*)attn_decode_kernel<DE_PLAIN, 8>,       (const void*)attn_decode_kernel<DE_TRACK, 8>,
-                            (const void*)attn_decode_kernel<DE_TRACK_AGAIN, 8>, (const void*)attn_decode_kernel<DE_PLAIN, 16>,
-                            (const void*)attn_decode_kernel<DE_TRACK, 16>,      (const void*)attn_decode_kernel<DE_TRACK_AGAIN, 16>};
-        for (const void* k : f) {
+        for (int i = 0; i < 18; i++) {
+            const DeKernel k = de_kernel(i < 9 ? 8 : 16, 1 << i / 3 % 3, i % 3);
+            if (!k) continue;
             if ((e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, DE_SMEM_MAX)) != cudaSuccess) return e;
             if ((e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
         }
@@ -345,50 +454,20 @@ cudaError_t launch_attn_decode(const AttnOp& a, cudaStream_t s) {
         a.window ? std::min(most, ((long long)a.window + 2 * AT_PAGE - 2) / AT_PAGE +
                                       std::min(most, ((long long)a.sinks + AT_PAGE - 1) / AT_PAGE))
                  : most;
-    // Splits: as many as fill the SMs once, two CTAs each, if there are pages
-    // enough to give each warp one. (64 x 4096 positions, 128 heads: 42 us in
-    // one part, 29 in two, 34 in four, 46 in eight.) Clusters of sixteen find
-    // place one at a time in each part of the chip: for few heads alone (8 x
-    // 4096, 16 heads: 10.4 us in eight parts, 16.5 in sixteen; 1 x 4096: 8.6
-    // and 7.6). Sixteen warps a CTA pay on a cache that gives each warp four
-    // pages (1 x 32768: 15.8 us against 18.9; 1 x 2048: 7.3 against 6.5).
-    const long long heads = (long long)a.seqs * a.kv_heads;
-    int ns = 1;
-    while (ns < DE_MAX_SPLIT && heads * ns * 2 <= (ns == 8 ? 64 : 2 * 148) && pages >= 2 * ns * 8) ns *= 2;
-    const int warps = heads * ns <= 64 && pages >= 4 * 16 * ns ? 16 : 8;
-    auto ld_of = [&](int ns) {  // 8 past a multiple of 32: the eight heads' stores fall on distinct banks
-        return (pages + ns - 1) / ns * AT_PAGE / 32 * 32 + 40;
-    };
-    auto track = [&](int ns) { return de_smem(warps) + ld_of(ns) * AT_MAXG * 4; };
-    int mode = DE_PLAIN, ld = 0;
-    size_t smem = de_smem(warps);
-    if (a.acc) {
-        // logits leave the L1 room for the loads in flight: with 86 KB of them
-        // a CTA (two parts) 64 x 4096 positions took 41.5 us, with 53 KB 38.4
-        while (ns < 8 && heads * ns > 148 && track(ns) > 56 * 1024) ns *= 2;
-        mode = track(ns) <= DE_SMEM_MAX ? DE_TRACK : DE_TRACK_AGAIN;
-        if (mode == DE_TRACK) {
-            smem = track(ns);
-            ld = (int)ld_of(ns);
-        }
-    }
+    const DePlan p = de_plan((long long)a.seqs * a.kv_heads, pages, a.acc != nullptr);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ns, a.kv_heads, a.seqs);
-    cfg.blockDim = dim3(warps * 32);
-    cfg.dynamicSmemBytes = smem;
+    cfg.gridDim = dim3(p.ns, a.kv_heads * p.parts, a.seqs);
+    cfg.blockDim = dim3(p.warps * 32);
+    cfg.dynamicSmemBytes = p.smem;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = ns;
+    at[0].val.clusterDim.x = p.ns;
     at[0].val.clusterDim.y = 1;
     at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    using Kernel = void (*)(AttnOp, int);
-    static const Kernel kernels[2][3] = {
-        {attn_decode_kernel<DE_PLAIN, 8>, attn_decode_kernel<DE_TRACK, 8>, attn_decode_kernel<DE_TRACK_AGAIN, 8>},
-        {attn_decode_kernel<DE_PLAIN, 16>, attn_decode_kernel<DE_TRACK, 16>, attn_decode_kernel<DE_TRACK_AGAIN, 16>}};
-    return cudaLaunchKernelEx(&cfg, kernels[warps == 16][mode], a, ld);
+    return cudaLaunchKernelEx(&cfg, de_kernel(p.warps, p.parts, p.mode), a, p.ld);
 }
 
 }  // namespace ming

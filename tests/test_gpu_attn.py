@@ -325,6 +325,19 @@ def test_decode_totals_of_caches_past_shared_memory(ctx, lens):
     check_decode(ctx, c)
 
 
+@pytest.mark.parametrize("lens,kvh", [
+    ([509], 2), ([130] * 3, 2), ([1000], 2), ([3000], 1), ([5000], 2), ([400, 0, 1, 399, 17, 33, 16, 250], 2), ([8200] * 2, 2),
+    (list(range(150, 509, 15)), 2), ([500] + [60] * 11, 2), ([3001, 0, 17, 2500], 2), ([2000] + [31] * 11, 2), ([700] * 3, 8),
+    ([120001], 1), ([120001], 2), ([50001] + list(range(9)), 2),
+], ids=lambda x: f"{len(x)}x{max(x)}" if isinstance(x, list) else str(x))
+def test_decode_divisions(ctx, lens, kvh):
+    """Few heads and many, short caches and long: pages and dims divided over
+    clusters of every size, with and without totals; groups of seven and one."""
+    check_decode(ctx, Case(lens, [1] * len(lens), 7 * kvh, kvh, 0, 0, seed=len(lens), poison=max(lens) < 10000))
+    if max(lens) < 10000:
+        check_decode(ctx, Case(lens, [1] * len(lens), kvh, kvh, 300, 5, layout="slot", seed=1))
+
+
 def test_one_row_of_a_prompt_is_a_token(ctx):
     """The two attention operators agree where they are the same thing."""
     c = Case([333, 40, 1], [1] * 3, 14, 2, 50, 4)
