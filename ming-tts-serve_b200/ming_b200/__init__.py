@@ -228,8 +228,9 @@ def _tensor(t, name, dtype, ndim, device):
     """Checks a device tensor; returns its strides, 0 for dimensions of one
     element, which are never strided over."""
     try:
-        if t.dtype is dtype and t.ndim == ndim and t.get_device() == device >= 0:
-            s, n = t.stride(), t.shape
+        s = t.stride()
+        if t.dtype is dtype and len(s) == ndim and t.get_device() == device >= 0:
+            n = t.shape
             if 1 not in n:
                 if s[-1] == 1:
                     return s
@@ -240,6 +241,30 @@ def _tensor(t, name, dtype, ndim, device):
                         f"on {t.device}")
     except AttributeError:
         raise MingError(f"{name}: a device tensor is wanted") from None
+
+
+def _heads(t, name, dtype, device):
+    """Shape, row and head stride of [rows, heads, 64] (_tensor's checks in fewer steps)."""
+    try:
+        n = t.shape
+        rows, heads, dims = n
+        r, h, e = t.stride()
+        if e == 1 and dims == 64 and t.dtype is dtype and t.get_device() == device:
+            return n, 0 if rows == 1 else r, 0 if heads == 1 else h
+    except (AttributeError, TypeError, ValueError):
+        pass
+    _tensor(t, name, dtype, 3, device)
+    raise MingError(f"{name}: heads of 64 dims are wanted")
+
+
+def _packed(t, name, dtype, shape, device):
+    """Checks a contiguous device tensor of a given shape; returns its address."""
+    try:
+        if t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        raise MingError(f"{name}: a device tensor is wanted") from None
+    raise MingError(f"{name}: contiguous {dtype} {list(shape)} on cuda:{device} is wanted")
 
 
 class KvCache:
@@ -272,11 +297,15 @@ class KvCache:
         """(address, seq, layer and head stride) of running totals f32 [seqs, layers, kv_heads, >= max_len]."""
         if acc is None:
             return 0, 0, 0, 0
-        s = _tensor(acc, name, _types()[1], 4, self.device)
-        *dims, n = acc.shape
-        if tuple(dims) != self.shape or n < self.max_len:
-            raise MingError(f"{name}: [seqs, layers, kv_heads, at least max_len] is wanted")
-        return acc.data_ptr(), s[0], s[1], s[2]
+        try:
+            n = acc.shape
+            a, b, c, e = acc.stride()
+            if (n[:3] == self.shape and n[3] >= self.max_len and (e == 1 or n[3] == 1) and acc.dtype is _types()[1]
+                    and acc.get_device() == self.device):
+                return acc.data_ptr(), a, b, c
+        except (AttributeError, TypeError, ValueError):
+            pass
+        raise MingError(f"{name}: f32 [seqs, layers, kv_heads, at least max_len] on the cache's device is wanted")
 
 
 # ming_attn and ming_evict, packed in one step (a structure's fields set one by
@@ -473,33 +502,24 @@ class Context:
         device = self.device
         if cache.device != device:
             raise MingError("the cache is on another device")
-        bf16, f32, i32 = _types()
-        r, h, _ = _tensor(q, "q", bf16, 3, device)
-        n = q.shape
-        rows, heads, dims = n
-        if dims != 64:
-            raise MingError("q: heads of 64 dims are wanted")
+        bf16, f32, i32 = _torch_types or _types()
+        n, r, h = _heads(q, "q", bf16, device)
+        rows, heads, _ = n
         o = o_r = o_h = start = z = a = a_s = a_l = a_h = 0
         if out is not None:
-            if out.shape != n:
+            shape, o_r, o_h = _heads(out, "out", bf16, device)
+            if shape != n:
                 raise MingError("out and q differ in shape")
-            o_r, o_h, _ = _tensor(out, "out", bf16, 3, device)
             o = out.data_ptr()
         if q_start is None:
             if rows != cache.seqs:
                 raise MingError("q: one row per sequence is wanted")
         else:
-            _tensor(q_start, "q_start", i32, 1, device)
-            if q_start.shape[0] != cache.seqs + 1:
-                raise MingError("q_start: seqs + 1 entries are wanted")
-            start = q_start.data_ptr()
+            start = _packed(q_start, "q_start", i32, (cache.seqs + 1,), device)
             if max_rows is None:
                 max_rows = rows
         if lse is not None:
-            _tensor(lse, "lse", f32, 2, device)
-            if lse.shape != n[:2] or not lse.is_contiguous():
-                raise MingError("lse: contiguous [rows, heads] is wanted")
-            z = lse.data_ptr()
+            z = _packed(lse, "lse", f32, (rows, heads), device)
         if acc is not None:
             a, a_s, a_l, a_h = cache._acc(acc)
         _ATTN.pack_into(self._args, 0, layer, heads, window, sinks, scale or 0.0, q.data_ptr(), r, h, o, o_r, o_h, start, rows,
@@ -545,13 +565,12 @@ class Context:
             raise MingError("the cache is on another device")
         i = 0
         if index is not None:
-            _tensor(index, "index", _types()[2], 4, self.device)
-            if index.shape != cache.shape + (keep,) or not index.is_contiguous():
-                raise MingError("index: contiguous [seqs, layers, kv_heads, keep] is wanted")
-            i = index.data_ptr()
+            i = _packed(index, "index", _types()[2], cache.shape + (keep,), self.device)
         _EVICT.pack_into(self._args, 0, keep, sinks, recent, *cache._acc(acc), *to._acc(acc_to, "acc_to"), i,
                          0 if stream is None else stream or 1)
-        _check(lib().ming_cuda_kv_evict(self._h, cache.ref, to.ref, self._args_at))
+        rc = _lib.ming_cuda_kv_evict(self._h, cache.ref, to.ref, self._args_at)
+        if rc:
+            _check(rc)
 
     def unpack_linear(self, weight_name, out_dim, in_dim):
         out = np.empty((out_dim, in_dim), dtype=np.float32)
