@@ -89,14 +89,14 @@ MING_DEV int at_len(const KvPages& kv, int n, int* err) {
     return n;
 }
 MING_DEV int at_len_of(const KvPages& kv, int seq, int* err) { return at_len(kv, kv.lens[seq] + kv.len_add, err); }
-// The page that holds page-index i of a sequence's table row, 0 if the entry
-// lies outside the pool.
-MING_DEV int at_page(const KvPages& kv, const int* row, int i, int* err) {
-    const int p = row[i];
-    if ((unsigned)p < (unsigned)kv.pages) return p;
+// The page of a table entry, 0 if it lies outside the pool; of page-index i of
+// a sequence's table row.
+MING_DEV int at_page_of(const KvPages& kv, int entry, int* err) {
+    if ((unsigned)entry < (unsigned)kv.pages) return entry;
     at_flag(err, AT_ERR_PAGE);
     return 0;
 }
+MING_DEV int at_page(const KvPages& kv, const int* row, int i, int* err) { return at_page_of(kv, row[i], err); }
 // A sequence's rows [r0, r1) of q as q_start gives them, clamped into [0, rows] and to max_rows.
 MING_DEV void at_rows(const AttnOp& a, int& r0, int& r1) {
     if (r0 < 0 || r1 > a.rows || r1 < r0 || r1 - r0 > a.max_rows) {

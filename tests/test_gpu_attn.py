@@ -238,6 +238,16 @@ def test_prefill_many_sequences(ctx, lens, window, sinks):
     check_prefill(ctx, Case(lens, [(n + 1) // 2 for n in lens], 16, 2, window, sinks, seed=len(lens)))
 
 
+@pytest.mark.parametrize("lens,rows,window,sinks", [
+    ([18] * 37, [18] * 37, 0, 0), ([128] * 37, [100] * 37, 0, 0), ([256] * 8, [256] * 8, 0, 0), ([1024] * 2, [1024, 40], 0, 0),
+    ([333], [333], 0, 0), ([1100], [256], 0, 0), ([509, 130, 1, 400], [509, 130, 1, 400], 128, 0), ([700, 20] * 4, [700, 20] * 4, 300, 5),
+    ([2048], [1900], 0, 0),
+], ids=lambda x: f"{len(x)}x{max(x)}" if isinstance(x, list) else str(x))
+def test_weights_divisions(ctx, lens, rows, window, sinks):
+    """Tiles of q divided over clusters of every size."""
+    check_prefill(ctx, Case(lens, rows, 14, 2, window, sinks, seed=2))
+
+
 def test_prefill_sharp(ctx):
     """Logits of hundreds: a row's weight sits on one or two positions and its maximum keeps rising."""
     check_prefill(ctx, Case([600], [600], 14, 2, 0, 0, sharp=60.0, seed=13))
