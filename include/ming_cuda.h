@@ -339,7 +339,8 @@ int ming_cuda_attn_decode(ming_ctx* ctx, const ming_kv_cache* cache, const ming_
  * `keep` positions stays whole. What stays moves, in order, to positions
  * 0, 1, .. of `to` (keys as they are: rotated for their first positions),
  * its totals to acc_to. index, unless NULL, receives the positions that
- * stayed, [seqs][layers][kv_heads][keep], -1 behind them. Each sequence then
+ * stayed, [seqs][layers][kv_heads][keep], -1 behind them. acc has max_len
+ * entries of each (sequence, layer, kv head). Each sequence then
  * holds min(len, keep) positions; lens is not written and to's is not read.
  * `to` may be `from` with acc_to = acc (in place); else the pages and totals
  * of the two do not overlap. A page that is written belongs to one sequence

@@ -13,6 +13,7 @@ constexpr int EV_WARPS = EV_THREADS / 32;
 constexpr int EV_BITS = 11;                 // radix of the selection: three digits of 11, 11 and 10 bits
 constexpr int EV_BINS = 1 << EV_BITS;
 constexpr int EV_AHEAD = 2;                 // rows of which a thread has a piece in flight
+constexpr int EV_OWN = 8;                   // totals that a thread keeps (4096 positions a CTA; more are read again)
 
 // Order-preserving key of a total: larger total, larger key. -0 counts as +0
 // and NaN as -infinity.
@@ -55,17 +56,37 @@ MING_DEV int ev_scan(int x, int lane) {  // inclusive
 template <int PARTS>
 __global__ void __launch_bounds__(EV_THREADS, 2) kv_evict_kernel(const EvictOp a) {
     extern __shared__ int ev_list[];  // positions that stay, ascending (when some between do and some do not)
-    __shared__ int hist[EV_BINS], warp_sum[EV_WARPS], warp_ties[EV_WARPS];
+    __shared__ __align__(16) int hist[EV_BINS];
+    __shared__ int warp_sum[EV_WARPS], warp_ties[EV_WARPS];
     __shared__ int s_digit, s_left, s_bin;
     constexpr int LANES = 8 / PARTS, ROWS = EV_THREADS / LANES;  // lanes of a row, rows at once
     const int part = blockIdx.x % PARTS, kh = blockIdx.x / PARTS, layer = blockIdx.y, b = blockIdx.z;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int seq = at_seq(a.from, b), n = at_len_of(a.from, seq, a.err), kept = min(a.keep, n);
+    const int seq = at_seq(a.from, b);
+    const float* acc = a.acc ? a.acc + seq * a.a_ss + layer * a.a_ls + kh * a.a_hs : nullptr;
+    const int* bt = a.from.bt + (size_t)seq * a.from.bt_ld;
+    const int* bt_to = a.to.bt + (size_t)seq * a.to.bt_ld;
+    // on their way together: the length, the totals and the tables (the latter for the L1)
+    const int held = a.from.lens[seq] + a.from.len_add;
+    float own[EV_OWN];
+    if (acc && a.sinks + a.recent < a.keep) {
+#pragma unroll
+        for (int i = 0; i < EV_OWN; i++) {
+            const int j = a.sinks + i * EV_THREADS + tid;
+            own[i] = j < a.from.max_len ? acc[j] : 0.f;
+        }
+    }
+    const int warm = (tid < a.from.bt_ld ? bt[tid] : 0) ^ (tid < a.to.bt_ld ? bt_to[tid] : 0);
+    const int n = at_len(a.from, held, a.err), kept = min(a.keep, n);
     const int lo = min(a.sinks, n), hi = max(lo, n - a.recent);
     const int need = n > a.keep ? a.keep - lo - (n - hi) : hi - lo;  // of the positions [lo, hi) between
-    const float* acc = a.acc ? a.acc + seq * a.a_ss + layer * a.a_ls + kh * a.a_hs : nullptr;
     const bool some = need > 0 && need < hi - lo;
-    if (some) {
+    if (some) {  // then n > keep, and lo is a.sinks
+        const int m = hi - lo;
+        const bool kept_here = m <= EV_OWN * EV_THREADS;  // every key is in its thread's registers
+        uint32_t key[EV_OWN];
+#pragma unroll
+        for (int i = 0; i < EV_OWN; i++) key[i] = ev_key(own[i]);
         // keys above `cut` stay, and the first `ties` of those at it; after an
         // early end, every key from `cut` on
         uint32_t cut = 0;
@@ -75,9 +96,15 @@ __global__ void __launch_bounds__(EV_THREADS, 2) kv_evict_kernel(const EvictOp a
             shift -= bits;
             for (int i = tid; i < EV_BINS; i += EV_THREADS) hist[i] = 0;
             __syncthreads();
-            for (int j = lo + tid; j < hi; j += EV_THREADS) {
-                const uint32_t k = ev_key(acc[j]);
+            auto count = [&](uint32_t k) {
                 if (pass == 0 || (k >> above) == cut) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1);
+            };
+            if (kept_here) {
+#pragma unroll
+                for (int i = 0; i < EV_OWN; i++)
+                    if (i * EV_THREADS + tid < m) count(key[i]);
+            } else {
+                for (int j = lo + tid; j < hi; j += EV_THREADS) count(ev_key(acc[j]));
             }
             __syncthreads();
             // thread t holds bins from the top: the digit is where the sum reaches `ties`
@@ -106,75 +133,109 @@ __global__ void __launch_bounds__(EV_THREADS, 2) kv_evict_kernel(const EvictOp a
         const bool whole = s_bin == ties;  // keys >= cut stay
         auto gt = [&](uint32_t k) { return whole ? k >= cut : k > cut; };
         auto eq = [&](uint32_t k) { return !whole && k == cut; };
-        // a warp's stretch of [lo, hi), in whole warps
-        const int per = ((hi - lo + EV_THREADS - 1) / EV_THREADS) * 32;
-        const int w0 = min(hi, lo + warp * per), w1 = min(hi, w0 + per);
-        int gts = 0, eqs = 0;
-        for (int j = w0 + lane; j < w1; j += 32) {
-            const uint32_t k = ev_key(acc[j]);
-            gts += gt(k);
-            eqs += eq(k);
-        }
-        gts = __reduce_add_sync(0xffffffffu, gts);
-        eqs = __reduce_add_sync(0xffffffffu, eqs);
-        __syncthreads();  // warp_sum's readers are done
-        if (lane == 0) {
-            warp_sum[warp] = gts;
-            warp_ties[warp] = eqs;
-        }
-        __syncthreads();
-        int at = lo, seen = 0;  // list place of the warp's first kept position; ties before it
-        for (int w = 0; w < warp; w++) {
-            at += warp_sum[w] + min(warp_ties[w], max(0, ties - seen));
-            seen += warp_ties[w];
-        }
-        for (int j = w0; j < w1; j += 32) {
-            const bool in = j + lane < w1;
-            const uint32_t k = in ? ev_key(acc[j + lane]) : 0;
-            const unsigned e = __ballot_sync(0xffffffffu, in && eq(k)), below = (1u << lane) - 1;
-            const bool stays = in && (gt(k) || (eq(k) && seen + __popc(e & below) < ties));
-            const unsigned s = __ballot_sync(0xffffffffu, stays);
-            if (stays) ev_list[at + __popc(s & below)] = j + lane;
-            at += __popc(s);
-            seen += __popc(e);
+        if (kept_here) {
+            // keys above the cut and ties, counted per (i, warp), which is their order
+            uint32_t above = 0, tie = 0;  // a bit per own key
+#pragma unroll
+            for (int i = 0; i < EV_OWN; i++) {
+                if (i * EV_THREADS >= m) break;
+                const bool in = i * EV_THREADS + tid < m, g = in && gt(key[i]), e = in && eq(key[i]);
+                const int c = __popc(__ballot_sync(0xffffffffu, g)) | __popc(__ballot_sync(0xffffffffu, e)) << 16;
+                if (lane == 0) hist[i * EV_WARPS + warp] = c;
+                above |= (uint32_t)g << i;
+                tie |= (uint32_t)e << i;
+            }
+            __syncthreads();
+            if (warp == 0) {  // both counts of the 128 before each, 4096 at most, in one sum
+                static_assert(EV_OWN * EV_WARPS == 128 && EV_OWN * EV_THREADS < 65536, "four counts a lane, packed");
+                int4 c = reinterpret_cast<int4*>(hist)[lane];
+                const int sum = (c.x + c.y) + (c.z + c.w), before = ev_scan(sum, lane) - sum;
+                reinterpret_cast<int4*>(hist)[lane] = make_int4(before, before + c.x, before + c.x + c.y, before + c.x + c.y + c.z);
+            }
+            __syncthreads();
+            const unsigned below = (1u << lane) - 1;
+#pragma unroll
+            for (int i = 0; i < EV_OWN; i++) {
+                if (i * EV_THREADS >= m) break;
+                const int c = hist[i * EV_WARPS + warp];
+                const bool g = (above >> i) & 1, e = (tie >> i) & 1;
+                const int gts = (c & 0xffff) + __popc(__ballot_sync(0xffffffffu, g) & below);
+                const int eqs = (c >> 16) + __popc(__ballot_sync(0xffffffffu, e) & below);
+                if (g || (e && eqs < ties)) ev_list[lo + gts + min(eqs, ties)] = lo + i * EV_THREADS + tid;
+            }
+        } else {
+            // a warp's stretch of [lo, hi), in whole warps
+            const int per = ((hi - lo + EV_THREADS - 1) / EV_THREADS) * 32;
+            const int w0 = min(hi, lo + warp * per), w1 = min(hi, w0 + per);
+            int gts = 0, eqs = 0;
+            for (int j = w0 + lane; j < w1; j += 32) {
+                const uint32_t k = ev_key(acc[j]);
+                gts += gt(k);
+                eqs += eq(k);
+            }
+            gts = __reduce_add_sync(0xffffffffu, gts);
+            eqs = __reduce_add_sync(0xffffffffu, eqs);
+            __syncthreads();  // warp_sum's readers are done
+            if (lane == 0) {
+                warp_sum[warp] = gts;
+                warp_ties[warp] = eqs;
+            }
+            __syncthreads();
+            int at = lo, seen = 0;  // list place of the warp's first kept position; ties before it
+            for (int w = 0; w < warp; w++) {
+                at += warp_sum[w] + min(warp_ties[w], max(0, ties - seen));
+                seen += warp_ties[w];
+            }
+            for (int j = w0; j < w1; j += 32) {
+                const bool in = j + lane < w1;
+                const uint32_t k = in ? ev_key(acc[j + lane]) : 0;
+                const unsigned e = __ballot_sync(0xffffffffu, in && eq(k)), below = (1u << lane) - 1;
+                const bool stays = in && (gt(k) || (eq(k) && seen + __popc(e & below) < ties));
+                const unsigned s = __ballot_sync(0xffffffffu, stays);
+                if (stays) ev_list[at + __popc(s & below)] = j + lane;
+                at += __popc(s);
+                seen += __popc(e);
+            }
         }
         __syncthreads();
     }
-    // everyone has read the totals: they may be overwritten behind the matching wait
-    if (acc && PARTS > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+    asm volatile("" ::"r"(warm));
+    // Everyone has read the totals (their values are in the list): they may be
+    // overwritten behind the matching wait. Nothing was written that another CTA reads.
+    if (acc && PARTS > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");
     // the position that moves to place s
     const int skipped = n - kept;
     auto source = [&](int s) { return s < lo ? s : s >= kept - (n - hi) || !some ? s + (s < lo + need ? 0 : skipped) : ev_list[s]; };
 
-    const int* bt = a.from.bt + (size_t)seq * a.from.bt_ld;
-    const int* bt_to = a.to.bt + (size_t)seq * a.to.bt_ld;
     const int col = part * (AT_HD / PARTS) + (tid % LANES) * 8, row = tid / LANES;
     const int64_t from0 = layer * a.from_ls + kh * a.from.hs + col, to0 = layer * a.to_ls + kh * a.to.hs + col;
     const bool in_place = a.from.k == a.to.k && a.from.v == a.to.v && bt == bt_to;
-    auto read = [&](int s0, uint4 (&v)[EV_AHEAD][2]) {
+    auto read = [&](int s0, uint4 (&v)[EV_AHEAD][2], int (&to)[EV_AHEAD]) {
 #pragma unroll
         for (int i = 0; i < EV_AHEAD; i++) {
             const int s = s0 + i * ROWS + row;
             if (s >= kept) continue;
             const int p = source(s);
+            to[i] = bt_to[s / AT_PAGE];
             const int64_t at = from0 + (int64_t)at_page(a.from, bt, p / AT_PAGE, a.err) * a.from.ps + (p % AT_PAGE) * a.from.ss;
             v[i][0] = *reinterpret_cast<const uint4*>(a.from.k + at);
             v[i][1] = *reinterpret_cast<const uint4*>(a.from.v + at);
         }
     };
     uint4 v[EV_AHEAD][2], w[EV_AHEAD][2];
+    int v_to[EV_AHEAD], w_to[EV_AHEAD];
     // in place, the first places often are the positions themselves
     int s0 = in_place ? lo / (EV_AHEAD * ROWS) * (EV_AHEAD * ROWS) : 0;
     if (in_place && skipped == 0) s0 = kept;
-    if (s0 < kept) read(s0, v);
+    if (s0 < kept) read(s0, v, v_to);
     for (; s0 < kept; s0 += EV_AHEAD * ROWS) {
         __syncthreads();  // the batch is read
-        if (s0 + EV_AHEAD * ROWS < kept) read(s0 + EV_AHEAD * ROWS, w);
+        if (s0 + EV_AHEAD * ROWS < kept) read(s0 + EV_AHEAD * ROWS, w, w_to);
 #pragma unroll
         for (int i = 0; i < EV_AHEAD; i++) {
             const int s = s0 + i * ROWS + row;
             if (s >= kept) continue;
-            const int page = bt_to[s / AT_PAGE];
+            const int page = v_to[i];
             if ((unsigned)page < (unsigned)a.to.pages) {
                 const int64_t at = to0 + (int64_t)page * a.to.ps + (s % AT_PAGE) * a.to.ss;
                 *reinterpret_cast<uint4*>(a.to.k + at) = v[i][0];
@@ -184,7 +245,7 @@ __global__ void __launch_bounds__(EV_THREADS, 2) kv_evict_kernel(const EvictOp a
             }
         }
 #pragma unroll
-        for (int i = 0; i < EV_AHEAD; i++) v[i][0] = w[i][0], v[i][1] = w[i][1];
+        for (int i = 0; i < EV_AHEAD; i++) v[i][0] = w[i][0], v[i][1] = w[i][1], v_to[i] = w_to[i];
     }
     if (part == 0 && a.index) {
         int* index = a.index + (((size_t)b * a.layers + layer) * a.kv_heads + kh) * a.keep;

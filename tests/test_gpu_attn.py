@@ -467,6 +467,13 @@ def test_evict(ctx, lens, keep, sinks, recent, kind, place):
     assert torch.equal(acc_to[~written].view(torch.int32), rest[2][~written].view(torch.int32))
 
 
+@pytest.mark.parametrize("n,sinks,recent", [(4096, 0, 0), (4097, 0, 0), (4097, 1, 0), (4099, 1, 2), (4100, 1, 2), (513, 1, 0), (514, 1, 0)])
+@pytest.mark.parametrize("kind", ["spread", "ties"])
+def test_evict_where_the_selection_changes(ctx, n, sinks, recent, kind):
+    """As many positions to choose from as threads hold, and one more or less."""
+    test_evict(ctx, [n, 17, n - 1], 401, sinks, recent, kind, "same")
+
+
 @pytest.mark.parametrize("seqs,layers", [(1, 24), (2, 24), (8, 24), (5, 40)])
 @pytest.mark.parametrize("place", ["apart", "same"])
 def test_evict_many_heads(ctx, seqs, layers, place):
