@@ -43,16 +43,21 @@ MING_DEV int ev_scan(int x, int lane) {  // inclusive
 //  * The smallest total that stays is found digit by digit: a histogram in
 //    shared memory, scanned from the top; the search ends early when a bin is
 //    taken whole. Positions that tie with it stay from the lowest on.
-//  * A warp counts its stretch of the positions, eight counts are summed, and
-//    the warp writes its kept positions to the list: two passes, one barrier.
+//  * The list: a thread keeps the totals of every 512th position as keys in
+//    registers; counts of what stays per 32 positions are summed by one warp,
+//    and each thread writes its positions in their places. Above 4096
+//    positions a warp reads its stretch of the totals again, twice.
+//  * The length, the totals and the page tables are asked for together: a
+//    chain of dependent loads is what a short cache's eviction takes.
 //  * Rows move EV_AHEAD to a thread at a time, K and V together, read before they are
 //    written. A row's place is never behind it, so what a batch writes no
 //    later one reads, and the next batch is read meanwhile.
-// Bound by the kept rows' bytes in a batch of sequences, by the chain of
-// dependent loads (length, totals, three histograms, pages, rows) for one.
+// Bound by the kept rows' bytes in a batch of sequences, by the chain (totals,
+// three histograms, list, pages, rows) for one.
 // Measured (24 layers, 2 kv heads): 16 sequences of up to 4096 positions cut
-// to 1024 69.6 us, 4.6 TB/s; one of 777 cut to 512 9.9 us. K and V in CTAs of
-// their own: 76 us; 256 threads 73; one or four rows ahead 74 and 90.
+// to 1024 64.1 us, 5.0 TB/s; one of 777 cut to 512 9.0 us. With the totals
+// read for every step, 69.9 and 10.1 us; then K and V in CTAs of their own:
+// 76 us; 256 threads 73; one or four rows ahead 74 and 90.
 template <int PARTS>
 __global__ void __launch_bounds__(EV_THREADS, 2) kv_evict_kernel(const EvictOp a) {
     extern __shared__ int ev_list[];  // positions that stay, ascending (when some between do and some do not)
