@@ -57,7 +57,7 @@ MING_DEV int ev_scan(int x, int lane) {  // inclusive
 // Measured (24 layers, 2 kv heads): 16 sequences of up to 4096 positions cut
 // to 1024 64.1 us, 5.0 TB/s; one of 777 cut to 512 9.0 us. With the totals
 // read for every step, 69.9 and 10.1 us; then K and V in CTAs of their own:
-// 76 us; 256 threads 73; one or four rows ahead 74 and 90.
+// 76 us; 256 threads 73. One, three or four rows ahead: 71, 75 and 87 us.
 template <int PARTS>
 __global__ void __launch_bounds__(EV_THREADS, 2) kv_evict_kernel(const EvictOp a) {
     extern __shared__ int ev_list[];  // positions that stay, ascending (when some between do and some do not)
