@@ -69,6 +69,12 @@ cudaError_t launch_attn_weights(const AttnOp& a, cudaStream_t s);
 cudaError_t launch_attn_decode(const AttnOp& a, cudaStream_t s);
 cudaError_t launch_kv_evict(const EvictOp& a, cudaStream_t s);
 
+// 2^x; what is below the smallest normal f32 becomes zero
+MING_DEV float at_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
 // Two f32 rounded to bf16 (to nearest, ties to even), lo in the low half.
 MING_DEV uint32_t at_bf16x2(float lo, float hi) {
     uint32_t r;

@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) attn_decode_kernel(con
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         if (__any_sync(0xffffffffu, mx > m)) {
-            const float mn = fmaxf(m, mx), r = exp2f(m - mn);
+            const float mn = fmaxf(m, mx), r = at_ex2(m - mn);
             m = mn;
             l *= r;
 #pragma unroll
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) attn_decode_kernel(con
         }
         float e[4];
 #pragma unroll
-        for (int d = 0; d < 4; d++) e[d] = exp2f(c[d] - m);
+        for (int d = 0; d < 4; d++) e[d] = at_ex2(c[d] - m);
         l += (e[0] + e[1]) + (e[2] + e[3]);
         const uint32_t h0 = at_bf16x2(e[0], e[1]), h1 = at_bf16x2(e[2], e[3]);
         const float2 f0 = unpack_bf16x2(h0), f1 = unpack_bf16x2(h1);
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) attn_decode_kernel(con
         float M = wm[at];
 #pragma unroll
         for (int i = 1; i < WARPS; i <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, i));
-        const float f = M == -INFINITY ? 0.f : exp2f(wm[at] - M);
+        const float f = M == -INFINITY ? 0.f : at_ex2(wm[at] - M);
         float L = wl[at] * f, x[OWN] = {};
 #pragma unroll
         for (int i = 1; i < WARPS; i <<= 1) L += __shfl_xor_sync(0xffffffffu, L, i);
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) attn_decode_kernel(con
             for (int r = 1; r < N; r++) M = fmaxf(M, f[r]);
 #pragma unroll
             for (int r = 0; r < N; r++) {
-                f[r] = M == -INFINITY ? 0.f : exp2f(f[r] - M);
+                f[r] = M == -INFINITY ? 0.f : at_ex2(f[r] - M);
                 L += l[r] * f[r];
             }
         };
@@ -328,15 +328,14 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) attn_decode_kernel(con
         __syncthreads();
         if (MODE == DE_TRACK) {
             for (int e0 = tid; e0 < mine; e0 += 4 * THREADS) {
-                float now[4];
+                float w[4] = {0.f, 0.f, 0.f, 0.f}, now[4];
+                for (int h = 0; h < a.group; h++) {
+                    const float M = fm[h], il = fl[h];
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int e = e0 + k * THREADS;
-                    float w = 0.f;
-                    if (e < mine)
-                        for (int h = 0; h < a.group; h++) w += exp2f(sc[h * sc_ld + e] - fm[h]) * fl[h];
-                    now[k] = old[k] + w;
+                    for (int k = 0; k < 4; k++) w[k] += at_ex2(sc[h * sc_ld + min(e0 + k * THREADS, mine - 1)] - M) * il;
                 }
+#pragma unroll
+                for (int k = 0; k < 4; k++) now[k] = old[k] + w[k];
                 fetch_acc(e0 + 4 * THREADS);
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
@@ -355,7 +354,7 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) attn_decode_kernel(con
                 logits(kf, p, c);
 #pragma unroll
                 for (int d = 0; d < 4; d++) {
-                    float w = g < a.group ? exp2f(c[d] - M) * il : 0.f;
+                    float w = g < a.group ? at_ex2(c[d] - M) * il : 0.f;
 #pragma unroll
                     for (int s = 4; s < 32; s <<= 1) w += __shfl_xor_sync(0xffffffffu, w, s);
                     const int j = p * AT_PAGE + 2 * t + (d & 1) + 4 * (d & 2);

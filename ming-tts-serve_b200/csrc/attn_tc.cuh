@@ -109,11 +109,6 @@ MING_DEV void at_wait_ld(uint32_t (&v)[N]) {
 }
 MING_DEV void at_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 
-MING_DEV float at_ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-    return y;
-}
 // Two f32 operations in one instruction
 MING_DEV uint64_t at_pair(float x, float y) {
     uint64_t r;
