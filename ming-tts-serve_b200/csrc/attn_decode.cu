@@ -69,9 +69,9 @@ MING_DEV uint32_t de_prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_
 // Bound by: the cache's bytes (256 per position and kv head) for batches, the
 // launch, two dependent loads and the cluster's two barriers for short rows,
 // what one SM takes in (some 65 GB/s) for few heads.
-// Measured (14 query, 2 kv heads): 64 x 4096 positions 27.9 us, 4.8 TB/s, and
-// 37.1 us with tracking (its logits take the L1's room from the loads in
-// flight); 1 x 509 4.2 us; 1 x 32768 10.3 us. Rings of cp.async three pages
+// Measured (14 query, 2 kv heads): 64 x 4096 positions 27.5 us, 4.9 TB/s, and
+// 37.5 us with tracking (its logits take the L1's room from the loads in
+// flight); 1 x 509 4.2 us; 1 x 32768 10.0 us. Rings of cp.async three pages
 // ahead and operands swapped for half the products changed none of this (34,
 // 42 and 18 us against 29, 38 and 16 at the time).
 template <int MODE, int WARPS, int PARTS>

@@ -147,7 +147,7 @@ struct PfRows {
 // tile's 128 x 128 weights, twice its products' 550. Measured: 16 prompts of
 // 2048 rows (14 query, 2 kv heads, causal) 191 us, 629 TFLOP/s, the
 // exponential unit 62% busy, the tensor pipe 31%, a block of both tiles 2570
-// cycles; one prompt of 128 rows 7.3 us, all latency. Tried and slower at that
+// cycles; one prompt of 128 rows 7.6 us, all latency. Tried and slower at that
 // size: a polynomial on the multiply-add pipes for a quarter of the weights
 // (218 us against 200), two threads a row (250), weights against the maximum
 // so far with a second pass where it rose (247), unrolled code beyond one body
